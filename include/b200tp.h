@@ -38,6 +38,7 @@ extern "C" {
 #define B200TP_ERR_WORKSPACE 5         /* workspace missing, misaligned or too small */
 #define B200TP_ERR_CUDA 6              /* a CUDA runtime / driver call failed */
 #define B200TP_ERR_NO_DEVICE 7         /* current device is not compute capability 10.x */
+#define B200TP_ERR_OPTIM_INPUT 8       /* maps to OptimizerInputError */
 
 /* device-side status words (written into `status`) */
 #define B200TP_DEV_TIMEOUT_PRODUCER 101
@@ -325,6 +326,101 @@ int b200tp_qk_norm_rope_fwd(const b200tp_prestep_args* a, const void* x, void* y
 size_t b200tp_qk_norm_rope_bwd_workspace_bytes(const b200tp_prestep_args* a);
 int b200tp_qk_norm_rope_bwd(const b200tp_prestep_args* a, const void* x, const void* dy, void* dx, float* d_weight,
                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Objectives over per-token log-probabilities
+ * ------------------------------------------------------------------------------------- */
+
+#define B200TP_PREFERENCE_SIGMOID 0
+#define B200TP_PREFERENCE_HINGE 1
+#define B200TP_PREFERENCE_SQUARED 2
+#define B200TP_KL_K1 0
+#define B200TP_KL_K2 1
+#define B200TP_KL_K3 2
+#define B200TP_NORMALIZE_TOKEN 0
+#define B200TP_NORMALIZE_SEQUENCE 1
+#define B200TP_NORMALIZE_SUM 2
+
+typedef struct b200tp_objective_args {
+  /* Tokens of `seqs` sequences.  cu_seqlens NULL: rows of `length` tokens, element i of sequence s at
+   * s * stride + i.  Else `length` packed tokens, sequence s being [cu[s], cu[s + 1]) of them (int32 or int64,
+   * seqs + 1 entries, rising); the strides are then 0. */
+  const void* logps;     /* `dtype`: log-probabilities of the trained model, or its losses -log p (from_nll) */
+  const void* old_logps; /* `other_dtype`: the sampling model's (policy loss) */
+  const void* ref_logps; /* `other_dtype`: the reference model's, or NULL */
+  const void* mask;      /* bytes, 0 leaves a token out whatever it holds; NULL takes all */
+  const void* advantages; /* f32 (policy loss): element at s * advantage_stride_seq + i * advantage_stride_token */
+  const void* cu_seqlens;
+  int64_t seqs, length;
+  int64_t logps_stride, old_stride, ref_stride, mask_stride;
+  int64_t advantage_stride_seq, advantage_stride_token;
+  int32_t dtype, other_dtype;
+  int32_t cu_is_int64;
+  int32_t from_nll;      /* 1: all log-probabilities are given as losses, and so is the gradient */
+} b200tp_objective_args;
+
+/* Preference loss over pairs: sequence i is preferred to sequence seqs / 2 + i.  With l_s the sum (average: the mean) over
+ * the taken tokens of logps - ref_logps and h = beta (l_i - l_{seqs/2 + i}) - margin, the mean over pairs of
+ * (1 - e) log(1 + exp(-h)) + e log(1 + exp(h)) (sigmoid, e = label_smoothing), max(0, 1 - h) (hinge) or
+ * ((h - 1/2) / beta)^2 (squared).  loss: one f32; rewards: (seqs,) f32 beta l_s; weights: (seqs,) f32 for
+ * b200tp_objective_bwd (slopes NULL, per_sequence 1).  The reference has no counterpart. */
+size_t b200tp_objective_workspace_bytes(const b200tp_objective_args* a);
+int b200tp_preference_loss_fwd(const b200tp_objective_args* a, int32_t kind, double beta, double label_smoothing,
+                               double margin, int32_t average, float* loss, float* rewards, float* weights,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* Clipped policy loss: per taken token -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef kl, r = exp(logps -
+ * old_logps), kl of logps against ref_logps (K1: logps - ref, K2: half its square, K3: exp(-d) + d - 1 for
+ * that difference d); averaged over all taken tokens, over each sequence's and then the sequences, or summed.
+ * out3: loss, mean kl and share of clipped tokens, both over the taken tokens.  slopes (NULL: no gradient wanted): f32 a
+ * token, (seqs, length) or (length,); weights: f32, (seqs,) for NORMALIZE_SEQUENCE (then per_sequence 1), else (1,). */
+int b200tp_policy_loss_fwd(const b200tp_objective_args* a, double clip_low, double clip_high, double kl_coef, int32_t kl_kind,
+                           int32_t normalize, float* out3, float* slopes, float* weights, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* Gradient of either loss for logps (contiguous, `dtype`, every token written): upstream[0] * weight * slope, a taken
+ * token's slope being 1 where slopes is NULL; 0 for the others. */
+int b200tp_objective_bwd(const b200tp_objective_args* a, const float* slopes, const float* weights, int32_t per_sequence,
+                         const float* upstream, void* grad, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * AdamW step over many tensors
+ * ------------------------------------------------------------------------------------- */
+
+typedef struct b200tp_adamw_tensor {
+  const void* param;     /* `param_dtype`, contiguous; with masters only written, through param_out */
+  const void* grad;      /* `grad_dtype`, contiguous */
+  void* param_out;       /* may be `param` */
+  int64_t numel;
+  int64_t state_offset;  /* of its first element in the states: a multiple of 256 */
+} b200tp_adamw_tensor;
+
+typedef struct b200tp_adamw_args {
+  /* States, flat over all tensors, each tensor's share padded to a multiple of 256 elements (padding zero); 16-byte
+   * aligned; *_out may be the same buffers (a step in place) or others that do not overlap them.
+   * bits 32: exp_avg, exp_avg_sq f32.  bits 8: e4m3 codes of m and of sqrt(v), and scales (blocks of 256, 2) f32:
+   * m = code * scales[.][0], sqrt(v) = code * scales[.][1]. */
+  const void* exp_avg;
+  const void* exp_avg_sq;
+  const void* scales;
+  const float* master;   /* f32 masters of bf16 parameters, or NULL */
+  void* exp_avg_out;
+  void* exp_avg_sq_out;
+  void* scales_out;
+  float* master_out;
+  double lr, beta1, beta2, eps, weight_decay;
+  double grad_scale;             /* gradients are multiplied by it ... */
+  const float* grad_scale_ptr;   /* ... and by this device scalar, unless NULL (a clipping coefficient) */
+  int64_t step;                  /* of this step, from 1 */
+  int32_t param_dtype, grad_dtype;
+  int32_t bits;
+  int32_t reserved;              /* 0 */
+} b200tp_adamw_args;
+
+/* m = b1 m + (1 - b1) g; v = b2 v + (1 - b2) g g; p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps), in
+ * fp32, each stored value rounded once.  `tensors` is host memory, read before the call returns; up to 600 tensors a
+ * launch.  Tensors that share memory are refused. */
+int b200tp_adamw_step(const b200tp_adamw_args* a, const b200tp_adamw_tensor* tensors, int32_t count, void* stream);
 
 #ifdef __cplusplus
 }

@@ -13,7 +13,7 @@ from pathlib import Path
 import torch
 
 from mlx_train_perf_b200.errors import (
-    AttentionInputError, DeviceTimeoutError, LossInputError, NativeLibraryError,
+    AttentionInputError, DeviceTimeoutError, LossInputError, NativeLibraryError, OptimizerInputError,
     UnsupportedAttentionError, UnsupportedHeadError,
 )
 
@@ -25,6 +25,7 @@ IMPL = {"auto": 0, "kernel": 0, "tc": 1, "simt": 2}
 OK = 0
 ERR_LOSS_INPUT, ERR_UNSUPPORTED_HEAD, ERR_ATTN_INPUT, ERR_UNSUPPORTED_ATTN = 1, 2, 3, 4
 ERR_WORKSPACE, ERR_CUDA, ERR_NO_DEVICE = 5, 6, 7
+ERR_OPTIM_INPUT = 8
 
 
 class CeArgs(C.Structure):
@@ -58,6 +59,27 @@ class PrestepArgs(C.Structure):
         ("weight", C.c_void_p), ("eps", C.c_float),
         ("cos", C.c_void_p), ("sin", C.c_void_p),
         ("cs_dtype", C.c_int32), ("cs_stride_b", C.c_int64), ("cs_stride_l", C.c_int64),
+    ]
+
+
+class ObjectiveArgs(C.Structure):
+    _fields_ = [
+        ("logps", C.c_void_p), ("old_logps", C.c_void_p), ("ref_logps", C.c_void_p), ("mask", C.c_void_p),
+        ("advantages", C.c_void_p), ("cu_seqlens", C.c_void_p),
+        ("seqs", C.c_int64), ("length", C.c_int64),
+        ("logps_stride", C.c_int64), ("old_stride", C.c_int64), ("ref_stride", C.c_int64), ("mask_stride", C.c_int64),
+        ("advantage_stride_seq", C.c_int64), ("advantage_stride_token", C.c_int64),
+        ("dtype", C.c_int32), ("other_dtype", C.c_int32), ("cu_is_int64", C.c_int32), ("from_nll", C.c_int32),
+    ]
+
+
+class AdamwArgs(C.Structure):
+    _fields_ = [
+        ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("scales", C.c_void_p), ("master", C.c_void_p),
+        ("exp_avg_out", C.c_void_p), ("exp_avg_sq_out", C.c_void_p), ("scales_out", C.c_void_p), ("master_out", C.c_void_p),
+        ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
+        ("grad_scale", C.c_double), ("grad_scale_ptr", C.c_void_p), ("step", C.c_int64),
+        ("param_dtype", C.c_int32), ("grad_dtype", C.c_int32), ("bits", C.c_int32), ("reserved", C.c_int32),
     ]
 
 
@@ -118,6 +140,17 @@ SIGNATURES = {
     "b200tp_flash_bwd": (C.c_int, [C.POINTER(AttnArgs), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                    C.c_size_t, C.c_void_p, C.c_void_p]),
+    # the tensors: (count, 5) int64 rows param, grad, param_out, numel, state_offset
+    "b200tp_adamw_step": (C.c_int, [C.POINTER(AdamwArgs), C.c_void_p, C.c_int32, C.c_void_p]),
+    "b200tp_objective_workspace_bytes": (C.c_size_t, [C.POINTER(ObjectiveArgs)]),
+    "b200tp_preference_loss_fwd": (C.c_int, [C.POINTER(ObjectiveArgs), C.c_int32, C.c_double, C.c_double, C.c_double,
+                                             C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                             C.c_void_p]),
+    "b200tp_policy_loss_fwd": (C.c_int, [C.POINTER(ObjectiveArgs), C.c_double, C.c_double, C.c_double, C.c_int32,
+                                         C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                         C.c_void_p]),
+    "b200tp_objective_bwd": (C.c_int, [C.POINTER(ObjectiveArgs), C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p,
+                                       C.c_void_p, C.c_void_p]),
 }
 
 _lock = threading.Lock()
@@ -170,6 +203,7 @@ _ERRORS = {
     ERR_UNSUPPORTED_HEAD: UnsupportedHeadError,
     ERR_ATTN_INPUT: AttentionInputError,
     ERR_UNSUPPORTED_ATTN: UnsupportedAttentionError,
+    ERR_OPTIM_INPUT: OptimizerInputError,
     ERR_WORKSPACE: NativeLibraryError,
     ERR_CUDA: NativeLibraryError,
     ERR_NO_DEVICE: NativeLibraryError,

@@ -34,6 +34,8 @@ SOURCES = [
     "capi_attn.cu",
     "selftest.cu",
     "prestep.cu",
+    "objectives.cu",
+    "optim.cu",
 ]
 
 NVCC_FLAGS = [

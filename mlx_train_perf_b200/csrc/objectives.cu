@@ -1,0 +1,530 @@
+// Objectives over per-token log-probabilities: the preference loss over pairs of sequences and the clipped policy loss
+// with a KL term.  They stand behind the per-token losses of the vocabulary loss (core/loss.py:235-250 of the reference),
+// where the reference's own training code has only the masked mean (adapters/mlx_lm.py:212-215).
+//
+// Tokens lie as (S, L) rows with a row stride, or as T packed tokens whose sequences are the ranges
+// [cu[s], cu[s + 1]).  A token that its mask leaves out takes no part whatever it holds: values are selected, never
+// multiplied by zero.
+//
+// Both losses are one pass over the tokens, then one block that joins the sequences' sums, then (backward) one pass that
+// writes the gradient.  A token costs 9 to 21 bytes and a few dozen operations, so long batches are bound by HBM and the
+// usual ones by launches: the pass and the join are two launches, the second one programmatic, and nothing is zeroed
+// beforehand (no counter, no atomics: sums are formed in a fixed order, in double, since what is left after
+// advantages of both signs cancel is small beside the terms).
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "common.h"
+#include "ptx.cuh"
+
+namespace b200tp {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kJoinThreads = 1024;
+constexpr int kUnroll = 4;
+
+struct Tokens {
+  const void* cu;        // (S + 1) borders, or null: rows
+  int cu_i64;
+  long long seqs, length;            // length: of a row, or of all packed tokens
+  int splits;                        // blocks a sequence
+  long long x_stride, old_stride, ref_stride, mask_stride, adv_seq, adv_tok;
+  const unsigned char* mask;
+  float sign;                        // -1: the inputs are negative log-probabilities
+};
+
+struct PolicyRule {
+  float log_low, log_high;           // log(1 - clip_low), log(1 + clip_high)
+  float low, high;                   // 1 - clip_low, 1 + clip_high
+  float kl_coef;
+  int kl_kind;
+};
+
+// What a block knows of one sequence's share of tokens.
+struct alignas(32) Part {
+  double loss, kl;
+  int count, clipped;
+  double pad;
+};
+
+__device__ __forceinline__ float ld(const float* p) { return *p; }
+__device__ __forceinline__ float ld(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void st(float* p, float v) { *p = v; }
+__device__ __forceinline__ void st(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ long long border(const Tokens& t, long long s) {
+  const long long b = t.cu_i64 ? static_cast<const long long*>(t.cu)[s] : static_cast<const int*>(t.cu)[s];
+  return min(max(b, 0ll), t.length);
+}
+// Tokens [lo, hi) of block (s, k); borders that do not rise give empty sequences, never an access outside.
+__device__ __forceinline__ void share(const Tokens& t, long long s, int k, long long& lo, long long& hi) {
+  lo = 0;
+  hi = t.length;
+  if (t.cu != nullptr) {
+    lo = border(t, s);
+    hi = max(border(t, s + 1), lo);
+  }
+  const long long per = (hi - lo + t.splits - 1) / t.splits;
+  lo = min(lo + per * k, hi);
+  hi = min(lo + per, hi);
+}
+
+__device__ __forceinline__ bool taken(const Tokens& t, long long s, long long i) {
+  return t.mask == nullptr || t.mask[s * t.mask_stride + i] != 0;
+}
+
+template <int N, typename T>
+__device__ __forceinline__ T block_sum(T v, T* shared) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+  __syncthreads();
+  T sum = 0;
+#pragma unroll
+  for (int w = 0; w < N / 32; ++w) sum += shared[w];
+  return sum;
+}
+
+// exp(z) - 1 - z without the cancellation near zero: below a quarter the Taylor series to z^9 / 9!, whose first term left out
+// is 2 z^8 / 10! < 1e-11 of the sum.
+__device__ __forceinline__ float exp_minus_line(float z, float expm1_z) {
+  if (fabsf(z) >= 0.25f) return expm1_z - z;
+  float s = 1.f / 362880.f;
+  s = fmaf(s, z, 1.f / 40320.f);
+  s = fmaf(s, z, 1.f / 5040.f);
+  s = fmaf(s, z, 1.f / 720.f);
+  s = fmaf(s, z, 1.f / 120.f);
+  s = fmaf(s, z, 1.f / 24.f);
+  s = fmaf(s, z, 1.f / 6.f);
+  s = fmaf(s, z, 0.5f);
+  return s * z * z;
+}
+
+// Per token:  u = x - o, ratio = exp(u);  clipped iff A > 0 and u > log(1 + high), or A < 0 and u < log(1 - low), which is
+// where min(ratio A, clip(ratio) A) takes the constant (decided on u, an exact difference for near values, and not
+// on the rounded exponential);  f = -A (clipped ? bound : ratio) + c kl;  slope = (clipped ? 0 : -A ratio) + c kl'.
+// Slopes are kept without their weight (1 / count is known only after all tokens): 4 bytes written here and read
+// again by the backward, where computing them anew would read 13 or more.
+template <typename TX, typename TR, bool REF>
+__global__ void __launch_bounds__(kThreads)
+policy_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ old, const TR* __restrict__ ref,
+                     const float* __restrict__ adv, const Tokens t, const PolicyRule r, float* __restrict__ slopes,
+                     Part* __restrict__ parts) {
+  griddep_wait();
+  griddep_launch_dependents();
+  __shared__ double sums[kThreads / 32];
+  __shared__ int counts[kThreads / 32];
+  const long long s = blockIdx.x / t.splits;
+  const int k = static_cast<int>(blockIdx.x % t.splits);
+  const long long out_stride = t.cu != nullptr ? 0 : t.length;
+  if (s == t.seqs) {                 // packed tokens outside every sequence: no slope
+    if (slopes != nullptr && k == 0 && t.cu != nullptr) {
+      const long long first = border(t, 0), last = border(t, t.seqs);
+      for (long long i = threadIdx.x; i < first; i += kThreads) slopes[i] = 0.f;
+      for (long long i = max(first, last) + threadIdx.x; i < t.length; i += kThreads) slopes[i] = 0.f;
+    }
+    return;
+  }
+  long long lo, hi;
+  share(t, s, k, lo, hi);
+  double loss = 0., kl_sum = 0.;
+  int count = 0, clips = 0;
+  for (long long base = lo + threadIdx.x; base < hi; base += kThreads * kUnroll) {
+    float xv[kUnroll], ov[kUnroll], rv[kUnroll], av[kUnroll];
+    bool on[kUnroll];
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      const long long i = base + j * kThreads;
+      const bool in = i < hi;
+      const long long c = in ? i : lo;
+      on[j] = in && taken(t, s, c);
+      xv[j] = ld(x + s * t.x_stride + c);
+      ov[j] = ld(old + s * t.old_stride + c);
+      if constexpr (REF) rv[j] = ld(ref + s * t.ref_stride + c);
+      av[j] = adv[s * t.adv_seq + c * t.adv_tok];
+    }
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      const long long i = base + j * kThreads;
+      if (i >= hi) break;
+      float slope = 0.f;
+      if (on[j]) {
+        const float u = t.sign * (xv[j] - ov[j]), a = av[j];
+        const bool up = a > 0.f && u > r.log_high, down = a < 0.f && u < r.log_low, clipped = up || down;
+        const float gain = a * (clipped ? (up ? r.high : r.low) : expf(u));
+        slope = clipped ? 0.f : -gain;
+        float kl = 0.f;
+        if constexpr (REF) {
+          const float z = t.sign * (rv[j] - xv[j]);
+          float kl_slope;
+          if (r.kl_kind == B200TP_KL_K3) {
+            const float e = expm1f(z);
+            kl = exp_minus_line(z, e);
+            kl_slope = -e;
+          } else if (r.kl_kind == B200TP_KL_K2) {
+            kl = 0.5f * z * z;
+            kl_slope = -z;
+          } else {
+            kl = -z;
+            kl_slope = 1.f;
+          }
+          slope = fmaf(r.kl_coef, kl_slope, slope);
+          kl_sum += kl;
+        }
+        loss += fmaf(r.kl_coef, kl, -gain);
+        count += 1;
+        clips += clipped;
+      }
+      if (slopes != nullptr) slopes[s * out_stride + i] = t.sign * slope;
+    }
+  }
+  loss = block_sum<kThreads>(loss, sums);
+  if constexpr (REF) kl_sum = block_sum<kThreads>(kl_sum, sums);
+  count = block_sum<kThreads>(count, counts);
+  clips = block_sum<kThreads>(clips, counts);
+  if (threadIdx.x == 0) parts[blockIdx.x] = Part{loss, kl_sum, count, clips, 0.};
+}
+
+__device__ __forceinline__ Part joined(const Part* parts, const Tokens& t, long long s) {
+  Part p{0., 0., 0, 0, 0.};
+  for (int k = 0; k < t.splits; ++k) {
+    const Part q = parts[s * t.splits + k];
+    p.loss += q.loss;
+    p.kl += q.kl;
+    p.count += q.count;
+    p.clipped += q.clipped;
+  }
+  return p;
+}
+
+// One block: a sequence's parts to a thread, then the batch's sums.  512 sequences of two parts: 32 kB.
+__global__ void __launch_bounds__(kJoinThreads)
+policy_join_kernel(const Part* __restrict__ parts, const Tokens t, int normalize, float* __restrict__ weights,
+                   float* __restrict__ out3) {
+  griddep_wait();
+  griddep_launch_dependents();
+  __shared__ double sums[kJoinThreads / 32];
+  double loss = 0., kl = 0., count = 0., clipped = 0.;      // counts in double: exact to 2^53
+  for (long long s = threadIdx.x; s < t.seqs; s += kJoinThreads) {
+    const Part p = joined(parts, t, s);
+    double l = p.loss;
+    if (normalize == B200TP_NORMALIZE_SEQUENCE) {
+      const double w = 1. / (static_cast<double>(t.seqs) * max(p.count, 1));
+      l *= w;
+      weights[s] = static_cast<float>(w);
+    }
+    loss += l;
+    kl += p.kl;
+    count += p.count;
+    clipped += p.clipped;
+  }
+  loss = block_sum<kJoinThreads>(loss, sums);
+  kl = block_sum<kJoinThreads>(kl, sums);
+  count = block_sum<kJoinThreads>(count, sums);
+  clipped = block_sum<kJoinThreads>(clipped, sums);
+  if (threadIdx.x == 0) {
+    const double per = 1. / max(count, 1.);
+    if (normalize != B200TP_NORMALIZE_SEQUENCE) weights[0] = normalize == B200TP_NORMALIZE_TOKEN ? static_cast<float>(per) : 1.f;
+    out3[0] = static_cast<float>(normalize == B200TP_NORMALIZE_TOKEN ? loss * per : loss);
+    out3[1] = static_cast<float>(kl * per);
+    out3[2] = static_cast<float>(clipped * per);
+  }
+}
+
+// Sum of the masked log ratios x - r of a sequence's share.
+template <typename TX, typename TR, bool REF>
+__global__ void __launch_bounds__(kThreads)
+preference_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ ref, const Tokens t, Part* __restrict__ parts) {
+  griddep_wait();
+  griddep_launch_dependents();
+  __shared__ double sums[kThreads / 32];
+  __shared__ int counts[kThreads / 32];
+  const long long s = blockIdx.x / t.splits;
+  long long lo, hi;
+  share(t, s, static_cast<int>(blockIdx.x % t.splits), lo, hi);
+  double sum = 0.;
+  int count = 0;
+  for (long long base = lo + threadIdx.x; base < hi; base += kThreads * kUnroll) {
+    float xv[kUnroll], rv[kUnroll];
+    bool on[kUnroll];
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      const long long i = base + j * kThreads;
+      const long long c = i < hi ? i : lo;
+      on[j] = i < hi && taken(t, s, c);
+      xv[j] = ld(x + s * t.x_stride + c);
+      if constexpr (REF) rv[j] = ld(ref + s * t.ref_stride + c);
+    }
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      if (!on[j]) continue;
+      double v = xv[j];
+      if constexpr (REF) v -= rv[j];
+      sum += v;
+      count += 1;
+    }
+  }
+  sum = block_sum<kThreads>(sum, sums);
+  count = block_sum<kThreads>(count, counts);
+  if (threadIdx.x == 0) parts[blockIdx.x] = Part{sum * t.sign, 0., count, 0, 0.};
+}
+
+// One block: pair i is the sequences i and P + i.  h = beta (l_i - l_{P + i}) - margin; out: the loss, the S rewards
+// beta l_s, and for each sequence the weight that the loss's gradient gives every taken token of it.
+__global__ void __launch_bounds__(kJoinThreads)
+preference_join_kernel(const Part* __restrict__ parts, const Tokens t, int kind, double beta, double smoothing, double margin,
+                       int average, float* __restrict__ loss_out, float* __restrict__ rewards, float* __restrict__ weights) {
+  griddep_wait();
+  griddep_launch_dependents();
+  __shared__ double sums[kJoinThreads / 32];
+  const long long pairs = t.seqs / 2;
+  double total = 0.;
+  for (long long i = threadIdx.x; i < pairs; i += kJoinThreads) {
+    const Part c = joined(parts, t, i), r = joined(parts, t, pairs + i);
+    const double cs = average ? 1. / max(c.count, 1) : 1., rs = average ? 1. / max(r.count, 1) : 1.;
+    const double lc = c.loss * cs, lr = r.loss * rs;
+    const double h = beta * (lc - lr) - margin;
+    double f, slope;
+    if (kind == B200TP_PREFERENCE_SIGMOID) {
+      const double e = exp(-fabs(h)), tail = log1p(e);
+      f = (1. - smoothing) * (tail + max(-h, 0.)) + smoothing * (tail + max(h, 0.));
+      slope = smoothing - (h >= 0. ? e : 1.) / (1. + e);             // smoothing - sigmoid(-h)
+    } else if (kind == B200TP_PREFERENCE_HINGE) {
+      f = h > 1. ? 0. : 1. - h;
+      slope = h < 1. ? -1. : 0.;
+    } else {
+      const double off = (h - 0.5) / beta;
+      f = off * off;
+      slope = 2. * off / beta;
+    }
+    if (isnan(h)) f = slope = h;                                      // comparisons above would hide it
+    total += f;
+    const double w = t.sign * beta * slope / static_cast<double>(pairs);
+    weights[i] = static_cast<float>(w * cs);
+    weights[pairs + i] = static_cast<float>(-w * rs);
+    rewards[i] = static_cast<float>(beta * lc);
+    rewards[pairs + i] = static_cast<float>(beta * lr);
+  }
+  total = block_sum<kJoinThreads>(total, sums);
+  if (threadIdx.x == 0) *loss_out = static_cast<float>(total / static_cast<double>(pairs));
+}
+
+// grad = upstream * weight * (slopes ? slope : mask).  `per_seq`: a weight for each sequence, else one.
+template <typename TX, bool SLOPES>
+__global__ void __launch_bounds__(kThreads)
+objective_grad_kernel(const float* __restrict__ slopes, const float* __restrict__ weights, int per_seq,
+                      const float* __restrict__ upstream, const Tokens t, TX* __restrict__ grad) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const long long s = blockIdx.x / t.splits;
+  const int k = static_cast<int>(blockIdx.x % t.splits);
+  const long long out_stride = t.cu != nullptr ? 0 : t.length;
+  if (s == t.seqs) {
+    if (k == 0 && t.cu != nullptr) {
+      const long long first = border(t, 0), last = border(t, t.seqs);
+      for (long long i = threadIdx.x; i < first; i += kThreads) st(grad + i, 0.f);
+      for (long long i = max(first, last) + threadIdx.x; i < t.length; i += kThreads) st(grad + i, 0.f);
+    }
+    return;
+  }
+  long long lo, hi;
+  share(t, s, k, lo, hi);
+  const float w = *upstream * weights[per_seq ? s : 0];
+  for (long long base = lo + threadIdx.x; base < hi; base += kThreads * kUnroll) {
+    float v[kUnroll];
+    bool on[kUnroll];
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      const long long i = base + j * kThreads;
+      const long long c = i < hi ? i : lo;
+      on[j] = taken(t, s, c);
+      v[j] = SLOPES ? slopes[s * out_stride + c] : 1.f;
+    }
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      const long long i = base + j * kThreads;
+      if (i < hi) st(grad + s * out_stride + i, on[j] ? w * v[j] : 0.f);
+    }
+  }
+}
+
+// Blocks a sequence: about 2048 tokens each on average, at most eight blocks an SM in all and at most 512 a sequence.
+int splits_of(long long seqs, long long length, bool packed) {
+  const int64_t mean = packed ? ceil_div(length, seqs) : length;
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(512, 8ll * sm_count() / seqs));
+  return static_cast<int>(std::max<int64_t>(1, std::min(most, ceil_div(mean, 2048))));
+}
+
+int check(const b200tp_objective_args* a) {
+  if (a == nullptr) return fail(B200TP_ERR_LOSS_INPUT, "args is null");
+  if (a->seqs < 1 || a->seqs > (1ll << 26)) return fail(B200TP_ERR_LOSS_INPUT, "the number of sequences must lie in [1, 2^26]");
+  if (a->length < 0) return fail(B200TP_ERR_LOSS_INPUT, "negative length");
+  if (a->length > (1ll << 30)) return fail(B200TP_ERR_LOSS_INPUT, "a row (or the packed batch) holds at most 2^30 tokens");
+  if ((a->dtype != B200TP_F32 && a->dtype != B200TP_BF16) || (a->other_dtype != B200TP_F32 && a->other_dtype != B200TP_BF16))
+    return fail(B200TP_ERR_LOSS_INPUT, "log-probabilities must be fp32 or bf16");
+  if (a->logps == nullptr && a->length > 0) return fail(B200TP_ERR_LOSS_INPUT, "logps is null");
+  return B200TP_OK;
+}
+
+Tokens tokens(const b200tp_objective_args* a) {
+  Tokens t;
+  t.cu = a->cu_seqlens;
+  t.cu_i64 = a->cu_is_int64;
+  t.seqs = a->seqs;
+  t.length = a->length;
+  t.splits = splits_of(a->seqs, a->length, a->cu_seqlens != nullptr);
+  t.x_stride = a->logps_stride;
+  t.old_stride = a->old_stride;
+  t.ref_stride = a->ref_stride;
+  t.mask_stride = a->mask_stride;
+  t.adv_seq = a->advantage_stride_seq;
+  t.adv_tok = a->advantage_stride_token;
+  t.mask = static_cast<const unsigned char*>(a->mask);
+  t.sign = a->from_nll ? -1.f : 1.f;
+  return t;
+}
+
+unsigned blocks_of(const Tokens& t, bool outside) {
+  return static_cast<unsigned>(t.seqs * t.splits + (outside && t.cu != nullptr ? 1 : 0));
+}
+
+int check_workspace(const b200tp_objective_args* a, void* workspace, size_t bytes) {
+  const size_t need = b200tp_objective_workspace_bytes(a);
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 || bytes < need)
+    return fail(B200TP_ERR_WORKSPACE, "objective workspace missing, misaligned or smaller than " + std::to_string(need) + " bytes");
+  return B200TP_OK;
+}
+
+template <typename TX, typename TR>
+int launch_policy(const b200tp_objective_args* a, const Tokens& t, const PolicyRule& r, float* slopes, Part* parts,
+                  cudaStream_t stream) {
+  auto go = [&](auto kernel) {
+    return launch_pdl(kernel, dim3(blocks_of(t, slopes != nullptr)), dim3(kThreads), 0, stream, static_cast<const TX*>(a->logps),
+                      static_cast<const TR*>(a->old_logps), static_cast<const TR*>(a->ref_logps),
+                      static_cast<const float*>(a->advantages), t, r, slopes, parts);
+  };
+  B200TP_CUDA_OK(a->ref_logps != nullptr ? go(policy_tokens_kernel<TX, TR, true>) : go(policy_tokens_kernel<TX, TR, false>));
+  return B200TP_OK;
+}
+
+template <typename TX, typename TR>
+int launch_preference(const b200tp_objective_args* a, const Tokens& t, Part* parts, cudaStream_t stream) {
+  auto go = [&](auto kernel) {
+    return launch_pdl(kernel, dim3(blocks_of(t, false)), dim3(kThreads), 0, stream, static_cast<const TX*>(a->logps),
+                      static_cast<const TR*>(a->ref_logps), t, parts);
+  };
+  B200TP_CUDA_OK(a->ref_logps != nullptr ? go(preference_tokens_kernel<TX, TR, true>) : go(preference_tokens_kernel<TX, TR, false>));
+  return B200TP_OK;
+}
+
+}  // namespace
+}  // namespace b200tp
+
+using namespace b200tp;
+
+extern "C" {
+
+size_t b200tp_objective_workspace_bytes(const b200tp_objective_args* a) {
+  if (check(a) != B200TP_OK) return 0;
+  return align_up(static_cast<size_t>(a->seqs) * splits_of(a->seqs, a->length, a->cu_seqlens != nullptr) * sizeof(Part), 256);
+}
+
+int b200tp_preference_loss_fwd(const b200tp_objective_args* a, int32_t kind, double beta, double label_smoothing,
+                               double margin, int32_t average, float* loss, float* rewards, float* weights,
+                               void* workspace, size_t workspace_bytes, void* stream_v) {
+  int rc = check(a);
+  if (rc) return rc;
+  if (a->seqs % 2 != 0) return fail(B200TP_ERR_LOSS_INPUT, "a preference loss needs an even number of sequences");
+  if (kind != B200TP_PREFERENCE_SIGMOID && kind != B200TP_PREFERENCE_HINGE && kind != B200TP_PREFERENCE_SQUARED)
+    return fail(B200TP_ERR_LOSS_INPUT, "unknown kind of preference loss");
+  if (!(beta > 0.)) return fail(B200TP_ERR_LOSS_INPUT, "beta must be positive");
+  if (loss == nullptr || rewards == nullptr || weights == nullptr) return fail(B200TP_ERR_LOSS_INPUT, "null output");
+  rc = check_workspace(a, workspace, workspace_bytes);
+  if (rc) return rc;
+  rc = require_sm100();
+  if (rc) return rc;
+  const Tokens t = tokens(a);
+  Part* parts = static_cast<Part*>(workspace);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  if (a->dtype == B200TP_BF16)
+    rc = a->other_dtype == B200TP_BF16 ? launch_preference<__nv_bfloat16, __nv_bfloat16>(a, t, parts, stream)
+                                       : launch_preference<__nv_bfloat16, float>(a, t, parts, stream);
+  else
+    rc = a->other_dtype == B200TP_BF16 ? launch_preference<float, __nv_bfloat16>(a, t, parts, stream)
+                                       : launch_preference<float, float>(a, t, parts, stream);
+  if (rc) return rc;
+  B200TP_CUDA_OK(launch_pdl(preference_join_kernel, dim3(1), dim3(kJoinThreads), 0, stream, static_cast<const Part*>(parts), t, kind,
+                            beta, label_smoothing, margin, average, loss, rewards, weights));
+  return B200TP_OK;
+}
+
+int b200tp_policy_loss_fwd(const b200tp_objective_args* a, double clip_low, double clip_high, double kl_coef, int32_t kl_kind,
+                           int32_t normalize, float* out3, float* slopes, float* weights, void* workspace,
+                           size_t workspace_bytes, void* stream_v) {
+  int rc = check(a);
+  if (rc) return rc;
+  if (!(clip_low >= 0. && clip_low <= 1.) || !(clip_high >= 0.))
+    return fail(B200TP_ERR_LOSS_INPUT, "clip_low must lie in [0, 1] and clip_high must not be negative");
+  if (kl_kind < B200TP_KL_K1 || kl_kind > B200TP_KL_K3) return fail(B200TP_ERR_LOSS_INPUT, "unknown kind of KL term");
+  if (normalize < B200TP_NORMALIZE_TOKEN || normalize > B200TP_NORMALIZE_SUM)
+    return fail(B200TP_ERR_LOSS_INPUT, "unknown normalisation");
+  if (kl_coef != 0. && a->ref_logps == nullptr && a->length > 0) return fail(B200TP_ERR_LOSS_INPUT, "a KL term needs ref_logps");
+  if (out3 == nullptr || weights == nullptr) return fail(B200TP_ERR_LOSS_INPUT, "null output");
+  if (a->length > 0 && (a->old_logps == nullptr || a->advantages == nullptr))
+    return fail(B200TP_ERR_LOSS_INPUT, "old_logps / advantages is null");
+  rc = check_workspace(a, workspace, workspace_bytes);
+  if (rc) return rc;
+  rc = require_sm100();
+  if (rc) return rc;
+  const Tokens t = tokens(a);
+  PolicyRule r;
+  r.log_low = static_cast<float>(std::log1p(-clip_low));      // clip_low = 1: minus infinity, nothing lies below
+  r.log_high = static_cast<float>(std::log1p(clip_high));
+  r.low = static_cast<float>(1. - clip_low);
+  r.high = static_cast<float>(1. + clip_high);
+  r.kl_coef = static_cast<float>(kl_coef);
+  r.kl_kind = kl_kind;
+  Part* parts = static_cast<Part*>(workspace);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  if (a->dtype == B200TP_BF16)
+    rc = a->other_dtype == B200TP_BF16 ? launch_policy<__nv_bfloat16, __nv_bfloat16>(a, t, r, slopes, parts, stream)
+                                       : launch_policy<__nv_bfloat16, float>(a, t, r, slopes, parts, stream);
+  else
+    rc = a->other_dtype == B200TP_BF16 ? launch_policy<float, __nv_bfloat16>(a, t, r, slopes, parts, stream)
+                                       : launch_policy<float, float>(a, t, r, slopes, parts, stream);
+  if (rc) return rc;
+  B200TP_CUDA_OK(launch_pdl(policy_join_kernel, dim3(1), dim3(kJoinThreads), 0, stream, static_cast<const Part*>(parts), t, normalize,
+                            weights, out3));
+  return B200TP_OK;
+}
+
+int b200tp_objective_bwd(const b200tp_objective_args* a, const float* slopes, const float* weights, int32_t per_sequence,
+                         const float* upstream, void* grad, void* stream_v) {
+  int rc = check(a);
+  if (rc) return rc;
+  if (weights == nullptr || upstream == nullptr || (grad == nullptr && a->length > 0))
+    return fail(B200TP_ERR_LOSS_INPUT, "weights / upstream / grad is null");
+  rc = require_sm100();
+  if (rc) return rc;
+  const Tokens t = tokens(a);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  auto go = [&](auto kernel, auto* out) {
+    return launch_pdl(kernel, dim3(blocks_of(t, true)), dim3(kThreads), 0, stream, slopes, weights, per_sequence, upstream, t, out);
+  };
+  if (a->dtype == B200TP_BF16) {
+    auto* out = static_cast<__nv_bfloat16*>(grad);
+    B200TP_CUDA_OK(slopes != nullptr ? go(objective_grad_kernel<__nv_bfloat16, true>, out)
+                                     : go(objective_grad_kernel<__nv_bfloat16, false>, out));
+  } else {
+    auto* out = static_cast<float*>(grad);
+    B200TP_CUDA_OK(slopes != nullptr ? go(objective_grad_kernel<float, true>, out) : go(objective_grad_kernel<float, false>, out));
+  }
+  return B200TP_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,539 @@
+// One AdamW step over many tensors, moments in 32 or in 8 bits, with or without fp32 masters of bf16 parameters: what the
+// reference leaves to mlx.optimizers.AdamW (its train steps; plan/estimate.py:57-135 books the two moments).
+//
+// Everything is read once and written once: 28 bytes an element for bf16 parameters with fp32 masters and fp32 moments, 10 for
+// bf16 parameters with 8-bit moments.  HBM bounds the first.  The second leaves time for about 56 instructions an element at
+// HBM's rate, and written plainly (a rounded square root and quotient, selections for values that are not finite) it takes 79; so its
+// arithmetic works on pairs of fp32 values (fma.rn.f32x2), folds the scales into the factors, and tests a thread's eight
+// elements together for what is rare.
+//
+// The table of tensors travels in the launch's own parameters: no copy to the device, no workspace, nothing that two captured
+// graphs would share.  A CTA takes some thousands of elements of one tensor; a warp takes blocks of 256, the elements that share a scale.
+//
+// 8-bit moments.  m: e4m3 codes (to nearest), scale amax / 448 of the block.  v: e4m3 codes of sqrt(v), scale rmax / 448, rounded up
+// or down by a dither that is fixed by position and step: beta2 moves v by a thousandth a step, far less than half the
+// distance of two codes, and rounding to nearest would hold every v where it is.  A v that is not zero is never coded as
+// zero: the update divides by it.  An element one of whose moments is not finite gets NaN for both; the block's scales are
+// taken from the others.
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <type_traits>
+#include <vector>
+
+#include "common.h"
+#include "ptx.cuh"
+
+namespace b200tp {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlock = 256;                 // elements that share a scale; tensors start at multiples of it in the states
+constexpr int kRound = 4096;                // elements that a CTA loads at once: two blocks a warp
+// Elements of one CTA.  8-bit moments: one round (94 % of the measured copy rate at 789 M elements; two rounds need either 120
+// registers, 75 %, or spills, 84 %).  32 bits: two, which halves the searches of the table (unaligned tensors: 100 % against 92 %).
+template <int BITS>
+constexpr int kChunk = BITS == 8 ? kRound : 2 * kRound;
+constexpr int kTensors = 600;               // of one launch: 26 kB of its parameters
+constexpr int kFew = 48;                    // of the small form: 2 kB
+
+struct Rule {
+  float beta1, beta2, one_beta1, one_beta2;
+  float root_beta2, root_one_beta2;         // of beta2 and 1 - beta2
+  float eps, decay;                         // decay: 1 - lr weight_decay
+  float rate;                               // lr / (1 - beta1^t)
+  float root;                               // 1 / sqrt(1 - beta2^t)
+  float grad_scale;
+  const float* grad_scale_ptr;              // or null
+  unsigned step;
+};
+
+struct States {
+  const void* m;
+  const void* v;
+  const float2* scales;
+  const float* master;
+  void* m_out;
+  void* v_out;
+  float2* scales_out;
+  float* master_out;
+};
+
+template <int N>
+struct Table {
+  const void* p[N];
+  const void* g[N];
+  void* out[N];
+  long long numel[N];
+  long long at[N];                          // of the tensor's first element in the states
+  int first[N + 1];                         // chunk of the tensor's first element
+  int count;
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool vec, int n, float (&v)[8]) {
+  if (vec && n >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    } else {
+      const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(T) == 2) v[i] = i < n ? __bfloat162float(p[i]) : 0.f;
+      else v[i] = i < n ? p[i] : 0.f;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, bool vec, int n, const float (&v)[8]) {
+  if (vec && n >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      uint4 u;
+      __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      __stcs(reinterpret_cast<uint4*>(p), u);
+    } else {
+      __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+      __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(v[4], v[5], v[6], v[7]));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) {
+        if constexpr (sizeof(T) == 2) p[i] = __float2bfloat16_rn(v[i]);
+        else p[i] = v[i];
+      }
+  }
+}
+
+// Pairs of fp32 values, one instruction for two.
+struct alignas(8) Pair {
+  float x, y;
+};
+__device__ __forceinline__ unsigned long long bits_of(Pair a) {
+  unsigned long long u;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(u) : "f"(a.x), "f"(a.y));
+  return u;
+}
+__device__ __forceinline__ Pair pair_of(unsigned long long u) {
+  Pair a;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(u));
+  return a;
+}
+__device__ __forceinline__ Pair both(float v) { return Pair{v, v}; }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits_of(a)), "l"(bits_of(b)), "l"(bits_of(c)));
+  return pair_of(d);
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits_of(a)), "l"(bits_of(b)));
+  return pair_of(d);
+}
+__device__ __forceinline__ float rsqrt_ftz(float v) {
+  float q;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(v));
+  return q;
+}
+__device__ __forceinline__ float rcp_ftz(float v) {
+  float q;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(v));
+  return q;
+}
+
+// Two e4m3 codes of a word, the lower or the upper ones.
+__device__ __forceinline__ Pair decode2(uint32_t w, int upper) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(upper ? w >> 16 : w & 0xffffu), __NV_E4M3);
+  const float2 f = __half22float2(__half2(h));
+  return Pair{f.x, f.y};
+}
+
+// 32 mixed bits of a pair of positions and the step: xor-shifts and odd multipliers.
+__device__ __forceinline__ uint32_t mix(uint32_t pair, uint32_t step) {
+  uint32_t x = (pair + step * 0x3504F333u) * 0x1E3779B1u;
+  x = (x ^ (x >> 16)) * 0x7FEB352Du;
+  x = (x ^ (x >> 15)) * 0x046CA68Bu;
+  return x ^ (x >> 16);
+}
+
+// y >= 0 to the e4m3 value below or above, up with a probability of the distance (dither uniform in [0, 2^20)); not zero unless y
+// is.  Below 2^-6, where e4m3 values lie 2^-9 apart, 2^-6 is added first: sums in [2^-6, 2^-5) lie as far apart.
+__device__ __forceinline__ float dithered(float y, uint32_t dither) {
+  const float lift = y < 0x1p-6f ? 0x1p-6f : 0.f;
+  const uint32_t u = __float_as_uint(y + lift) + dither;
+  return fmaxf(__uint_as_float(u & 0xfff00000u) - lift, y > 0.f ? 0x1p-9f : 0.f);
+}
+
+// Eight elements as they lie in memory.
+template <typename T>
+struct Raw8 {
+  uint4 w[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ void fetch8(const T* p, bool vec, int n, Raw8<T>& r) {
+  if (vec && n >= 8) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) r.w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  } else {
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : T(0.f);
+    memcpy(&r, v, sizeof(v));
+  }
+}
+__device__ __forceinline__ void unpack(const Raw8<__nv_bfloat16>& r, Pair (&v)[4]) {
+  const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = Pair{__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u)};
+}
+__device__ __forceinline__ void unpack(const Raw8<float>& r, Pair (&v)[4]) {
+  v[0] = Pair{__uint_as_float(r.w[0].x), __uint_as_float(r.w[0].y)};
+  v[1] = Pair{__uint_as_float(r.w[0].z), __uint_as_float(r.w[0].w)};
+  v[2] = Pair{__uint_as_float(r.w[1].x), __uint_as_float(r.w[1].y)};
+  v[3] = Pair{__uint_as_float(r.w[1].z), __uint_as_float(r.w[1].w)};
+}
+
+// 8-bit moments of eight elements: (codes, scales) and gradients in, parameters moved, (codes, scales) out.
+// m = beta1 sm code + one_beta1 g;  v = (sqrt(beta2) sv code)^2 + (sqrt(one_beta2) g)^2, g times grad_scale;  sqrt(v) from v rsqrt(v) and
+// one Newton step (about an ulp; a v below 1e-37 counts as that small a one: its root is 0 or far below eps).
+__device__ __forceinline__ void step8(uint2& mc, uint2& vc, float2& sc, const Pair (&g)[4], Pair (&p)[4], float grad_scale,
+                                      const Rule& r, uint32_t position) {
+  Pair m[4], root[4];
+  const Pair bm = both(r.beta1 * sc.x), bv = both(r.root_beta2 * sc.y);
+  const Pair gm = both(r.one_beta1 * grad_scale), gr = both(r.root_one_beta2 * grad_scale);
+  float ma = 0.f;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const Pair cm = decode2(i < 2 ? mc.x : mc.y, i & 1), cv = decode2(i < 2 ? vc.x : vc.y, i & 1);
+    m[i] = fma2(g[i], gm, mul2(cm, bm));
+    const Pair new_root = mul2(g[i], gr), old_root = mul2(cv, bv);
+    const Pair v = fma2(new_root, new_root, mul2(old_root, old_root));
+    const Pair q = Pair{rsqrt_ftz(fmaxf(v.x, 1e-37f)), rsqrt_ftz(fmaxf(v.y, 1e-37f))};
+    const Pair t = mul2(v, q);
+    root[i] = fma2(Pair{fmaf(-t.x, t.x, v.x), fmaf(-t.y, t.y, v.y)}, mul2(q, both(0.5f)), t);
+    const Pair d = fma2(root[i], both(r.root), both(r.eps));
+    const Pair move = mul2(m[i], Pair{rcp_ftz(d.x), rcp_ftz(d.y)});
+    p[i] = fma2(move, both(-r.rate), mul2(p[i], both(r.decay)));
+    ma = fmaxf(ma, fmaxf(fabsf(m[i].x), fabsf(m[i].y)));
+    const Pair either = fma2(m[i], both(0.f), root[i]);             // the root, or NaN where either is not finite
+    top = max(top, max(__float_as_uint(either.x), __float_as_uint(either.y)));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);                        // by their bits: what is not finite lies above all else
+  const bool finite = top < 0x7f800000u;
+  if (!finite) {                                                    // rare: scales from the finite values alone
+    ma = 0.f;
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float& me = i & 1 ? m[i >> 1].y : m[i >> 1].x;
+      float& re = i & 1 ? root[i >> 1].y : root[i >> 1].x;
+      if (fabsf(me) < INFINITY && re < INFINITY) {
+        ma = fmaxf(ma, fabsf(me));
+        top = max(top, __float_as_uint(re));
+      } else {
+        me = re = NAN;
+      }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+  }
+  const float mm = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(ma))), rm = __uint_as_float(top);
+  // moments of 1e-30 and less are zero: their scale's reciprocal would overflow (a root is 0 or above 1e-23)
+  const Pair mi = both(mm > 1e-30f ? 448.f * rcp_ftz(mm) : 0.f), ri = both(rm > 0.f ? 448.f * rcp_ftz(rm) : 0.f);
+  sc = make_float2(mm > 1e-30f ? mm * (1.f / 448.f) : 0.f, rm * (1.f / 448.f));
+  uint32_t mw[4], vw[4], low = 0xffffffffu;
+  Pair y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const Pair x = mul2(m[i], mi);
+    mw[i] = __nv_cvt_float2_to_fp8x2(make_float2(x.x, x.y), __NV_SATFINITE, __NV_E4M3);
+    y[i] = mul2(root[i], ri);
+    low = min(low, min(__float_as_uint(y[i].x), __float_as_uint(y[i].y)));
+  }
+  mc = make_uint2(mw[0] | (mw[1] << 16), mw[2] | (mw[3] << 16));
+  const uint32_t pair = position >> 1;
+  if (finite && low >= 0x3c800000u) {
+    // All of the thread's y lie at 2^-6 or above: a code is its fp32 bits 20 to 26 after the dither and less the exponents' distance
+    // (120 << 23).  Times 16 they are the top byte: u * 16 + (dither * 16 - (120 << 27)), the latter put together from bytes.
+    // The largest dither is 8 short of a code's distance, and the largest y some 3 ulps above 448: never the code beyond, a NaN.
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t bits = mix(pair + i, r.step);
+      const uint32_t d0 = __byte_perm(bits, 0x00004080u, 0x5104), d1 = __byte_perm(bits, 0x00004080u, 0x5324);
+      h[i] = __byte_perm(__float_as_uint(y[i].x) * 16u + d0, __float_as_uint(y[i].y) * 16u + d1, 0x0073);
+    }
+    vc = make_uint2(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t bits = mix(pair + i, r.step);
+      float a = dithered(y[i].x, ((bits & 0xffffu) << 4) | 8u), b = dithered(y[i].y, ((bits >> 16) << 4) | 8u);
+      if (isnan(root[i].x)) a = NAN;
+      if (isnan(root[i].y)) b = NAN;
+      vw[i] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    }
+    vc = make_uint2(vw[0] | (vw[1] << 16), vw[2] | (vw[3] << 16));
+  }
+}
+
+template <typename TP, typename TG, int BITS, bool MASTER, int N>
+__global__ void __launch_bounds__(kThreads, 4)
+adamw_kernel(const __grid_constant__ Table<N> table, const States st, const Rule r) {
+  griddep_wait();
+  griddep_launch_dependents();
+  // the tensor of this chunk: the last one whose first chunk is not beyond it
+  const int chunk = blockIdx.x;
+  int lo = 0, hi = table.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (table.first[mid] <= chunk) lo = mid;
+    else hi = mid - 1;
+  }
+  const TP* p = static_cast<const TP*>(table.p[lo]);
+  const TG* g = static_cast<const TG*>(table.g[lo]);
+  TP* out = static_cast<TP*>(table.out[lo]);
+  const long long numel = table.numel[lo], at = table.at[lo];
+  const bool p_vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  const bool g_vec = (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+  const float grad_scale = r.grad_scale_ptr != nullptr ? r.grad_scale * *r.grad_scale_ptr : r.grad_scale;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long from = static_cast<long long>(chunk - table.first[lo]) * kChunk<BITS>, to = min(from + kChunk<BITS>, numel);
+
+  constexpr int kTimes = kRound / kThreads / 8;
+  if constexpr (BITS == 8) {
+    const long long start = from;
+    using TV = std::conditional_t<MASTER, float, TP>;               // what holds the value: the parameter or its master
+    // `whole`: every element of the chunk exists and every address is aligned, so nothing is asked per lane (3 instructions an
+    // element less); else lanes past the end load nothing and write nothing but the states' padding
+    auto chunk_of = [&](auto whole_t) {
+      constexpr bool whole = decltype(whole_t)::value;
+      Raw8<TG> gr[kTimes];
+      Raw8<TV> pr[kTimes];
+      uint2 mc[kTimes], vc[kTimes];
+      float2 sc[kTimes];
+      const long long i0 = start + threadIdx.x * 8, j0 = at + i0;   // warp w has block w, then block w + 8
+      const TG* gp = g + i0;
+      const TV* pp = MASTER ? reinterpret_cast<const TV*>(st.master + j0) : reinterpret_cast<const TV*>(p + i0);
+      const uint8_t* mp = static_cast<const uint8_t*>(st.m) + j0;
+      const uint8_t* vp = static_cast<const uint8_t*>(st.v) + j0;
+      const long long b0 = (at + start) / kBlock + warp;
+      auto left = [&](int it) { return numel - start - (it * (kThreads / 32) + warp) * kBlock; };   // elements from the warp's block on
+      auto mine = [&](int it) { return whole ? 8 : static_cast<int>(min(max(left(it) - lane * 8, 0ll), 8ll)); };
+#pragma unroll
+      for (int it = 0; it < kTimes; ++it) {                         // all loads first
+        if (!whole && left(it) <= 0) continue;                      // uniform in the warp
+        constexpr int kStep = kThreads * 8;
+        fetch8(gp + it * kStep, whole || g_vec, mine(it), gr[it]);
+        fetch8(pp + it * kStep, whole || MASTER || p_vec, MASTER ? 8 : mine(it), pr[it]);
+        mc[it] = __ldcs(reinterpret_cast<const uint2*>(mp + it * kStep));
+        vc[it] = __ldcs(reinterpret_cast<const uint2*>(vp + it * kStep));
+        sc[it] = st.scales[b0 + it * (kThreads / 32)];
+      }
+      TP* op = out + i0;
+#pragma unroll
+      for (int it = 0; it < kTimes; ++it) {
+        if (!whole && left(it) <= 0) continue;
+        constexpr int kStep = kThreads * 8;
+        Pair gv[4], pv[4];
+        unpack(gr[it], gv);
+        unpack(pr[it], pv);
+        step8(mc[it], vc[it], sc[it], gv, pv, grad_scale, r, static_cast<uint32_t>(j0) + it * kStep);
+        const float flat[8] = {pv[0].x, pv[0].y, pv[1].x, pv[1].y, pv[2].x, pv[2].y, pv[3].x, pv[3].y};
+        if constexpr (MASTER) store8(st.master_out + j0 + it * kStep, true, 8, flat);
+        store8(op + it * kStep, whole || p_vec, mine(it), flat);
+        __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.m_out) + j0 + it * kStep), mc[it]);
+        __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.v_out) + j0 + it * kStep), vc[it]);
+        if (lane == 0) st.scales_out[b0 + it * (kThreads / 32)] = sc[it];
+      }
+    };
+    if (start + kRound <= numel && p_vec && g_vec) chunk_of(std::true_type{});
+    else chunk_of(std::false_type{});
+  } else {
+#pragma unroll 1
+    for (long long start = from; start < to; start += kRound)
+#pragma unroll
+    for (int it = 0; it < kTimes; ++it) {
+      const long long block = start + (it * (kThreads / 32) + warp) * kBlock;
+      if (block >= numel) break;
+      const long long i = block + lane * 8, j = at + i;
+      const int n = static_cast<int>(min(max(numel - i, 0ll), 8ll));
+      float pv[8], gv[8], m[8], v[8];
+      load8(g + i, g_vec, n, gv);
+      if constexpr (MASTER) load8(st.master + j, true, 8, pv);
+      else load8(p + i, p_vec, n, pv);
+      load8(static_cast<const float*>(st.m) + j, true, 8, m);
+      load8(static_cast<const float*>(st.v) + j, true, 8, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = gv[e] * grad_scale;
+        m[e] = fmaf(r.beta1, m[e], r.one_beta1 * a);
+        v[e] = fmaf(r.beta2, v[e], r.one_beta2 * a * a);
+        pv[e] = fmaf(pv[e], r.decay, -r.rate * __fdividef(m[e], fmaf(sqrtf(v[e]), r.root, r.eps)));
+      }
+      if constexpr (MASTER) store8(st.master_out + j, true, 8, pv);
+      store8(out + i, p_vec, n, pv);
+      store8(static_cast<float*>(st.m_out) + j, true, 8, m);
+      store8(static_cast<float*>(st.v_out) + j, true, 8, v);
+    }
+  }
+}
+
+template <typename TP, typename TG, int BITS, bool MASTER, int N>
+int launch_n(const b200tp_adamw_tensor* t, int count, const States& st, const Rule& r, cudaStream_t stream) {
+  Table<N> table;
+  int chunks = 0, kept = 0;
+  for (int i = 0; i < count; ++i) {
+    if (t[i].numel == 0) continue;
+    table.p[kept] = t[i].param;
+    table.g[kept] = t[i].grad;
+    table.out[kept] = t[i].param_out;
+    table.numel[kept] = t[i].numel;
+    table.at[kept] = t[i].state_offset;
+    table.first[kept++] = chunks;
+    chunks += static_cast<int>(ceil_div(t[i].numel, kChunk<BITS>));
+  }
+  if (kept == 0) return B200TP_OK;
+  table.first[kept] = chunks;
+  table.count = kept;
+  B200TP_CUDA_OK(launch_pdl(adamw_kernel<TP, TG, BITS, MASTER, N>, dim3(chunks), dim3(kThreads), 0, stream, table, st, r));
+  return B200TP_OK;
+}
+
+// Few tensors to a launch: by their number, and by their chunks so that the grid and `first` stay in 31 bits.
+template <typename TP, typename TG, int BITS, bool MASTER>
+int launch_all(const b200tp_adamw_tensor* t, int count, const States& st, const Rule& r, cudaStream_t stream) {
+  int i = 0;
+  while (i < count) {
+    int n = 0;
+    int64_t chunks = 0;
+    while (i + n < count && n < kTensors && (n == 0 || chunks + ceil_div(t[i + n].numel, kChunk<BITS>) < (1ll << 31) - 1))
+      chunks += ceil_div(t[i + n++].numel, kChunk<BITS>);
+    const int rc = n <= kFew ? launch_n<TP, TG, BITS, MASTER, kFew>(t + i, n, st, r, stream)
+                             : launch_n<TP, TG, BITS, MASTER, kTensors>(t + i, n, st, r, stream);
+    if (rc) return rc;
+    i += n;
+  }
+  return B200TP_OK;
+}
+
+template <typename TP, typename TG>
+int launch_kind(const b200tp_adamw_args* a, const b200tp_adamw_tensor* t, int count, const States& st, const Rule& r,
+                cudaStream_t stream) {
+  if constexpr (sizeof(TP) == 2) {
+    if (a->master != nullptr)
+      return a->bits == 8 ? launch_all<TP, TG, 8, true>(t, count, st, r, stream) : launch_all<TP, TG, 32, true>(t, count, st, r, stream);
+  }
+  return a->bits == 8 ? launch_all<TP, TG, 8, false>(t, count, st, r, stream) : launch_all<TP, TG, 32, false>(t, count, st, r, stream);
+}
+
+bool misaligned(const void* p, unsigned mask) { return (reinterpret_cast<uintptr_t>(p) & mask) != 0; }
+
+// Two written ranges that overlap would race: the same tensor twice, or two views of one another.
+int check_apart(std::vector<std::pair<uintptr_t, uintptr_t>>& ranges, const char* what) {
+  std::sort(ranges.begin(), ranges.end());
+  for (size_t i = 1; i < ranges.size(); ++i)
+    if (ranges[i].first < ranges[i - 1].second)
+      return fail(B200TP_ERR_OPTIM_INPUT, std::string("two tensors of one step share memory (") + what + ")");
+  return B200TP_OK;
+}
+
+int check(const b200tp_adamw_args* a, const b200tp_adamw_tensor* t, int32_t count) {
+  if (a == nullptr || (t == nullptr && count > 0)) return fail(B200TP_ERR_OPTIM_INPUT, "args or the tensors are null");
+  if (count < 0) return fail(B200TP_ERR_OPTIM_INPUT, "negative number of tensors");
+  if ((a->param_dtype != B200TP_F32 && a->param_dtype != B200TP_BF16) || (a->grad_dtype != B200TP_F32 && a->grad_dtype != B200TP_BF16))
+    return fail(B200TP_ERR_OPTIM_INPUT, "parameters and gradients must be fp32 or bf16");
+  if (a->bits != 8 && a->bits != 32) return fail(B200TP_ERR_OPTIM_INPUT, "moments are kept in 8 or 32 bits");
+  if ((a->master == nullptr) != (a->master_out == nullptr)) return fail(B200TP_ERR_OPTIM_INPUT, "master and master_out go together");
+  if (a->master != nullptr && a->param_dtype == B200TP_F32) return fail(B200TP_ERR_OPTIM_INPUT, "fp32 parameters need no masters");
+  if (a->step < 1) return fail(B200TP_ERR_OPTIM_INPUT, "step counts from 1");
+  if (!(a->beta1 >= 0. && a->beta1 < 1.) || !(a->beta2 >= 0. && a->beta2 < 1.)) return fail(B200TP_ERR_OPTIM_INPUT, "betas must lie in [0, 1)");
+  if (!(a->eps >= 0.) || !(a->lr >= 0.) || !(a->weight_decay >= 0.))
+    return fail(B200TP_ERR_OPTIM_INPUT, "lr, eps and weight_decay must not be negative");
+  if (count > 0 && (a->exp_avg == nullptr || a->exp_avg_sq == nullptr || a->exp_avg_out == nullptr || a->exp_avg_sq_out == nullptr ||
+                    (a->bits == 8 && (a->scales == nullptr || a->scales_out == nullptr))))
+    return fail(B200TP_ERR_OPTIM_INPUT, "null states");
+  const void* states[] = {a->exp_avg, a->exp_avg_sq, a->scales, a->master, a->exp_avg_out, a->exp_avg_sq_out, a->scales_out, a->master_out};
+  for (const void* p : states)
+    if (misaligned(p, 15)) return fail(B200TP_ERR_OPTIM_INPUT, "states must be 16-byte aligned");
+  std::vector<std::pair<uintptr_t, uintptr_t>> written, offsets;
+  written.reserve(count);
+  offsets.reserve(count);
+  const unsigned p_item = a->param_dtype == B200TP_BF16 ? 2 : 4, g_item = a->grad_dtype == B200TP_BF16 ? 2 : 4;
+  for (int i = 0; i < count; ++i) {
+    if (t[i].numel < 0 || t[i].numel > (1ll << 42)) return fail(B200TP_ERR_OPTIM_INPUT, "bad number of elements");
+    if (t[i].numel == 0) continue;
+    if (t[i].param == nullptr || t[i].grad == nullptr || t[i].param_out == nullptr) return fail(B200TP_ERR_OPTIM_INPUT, "null tensor");
+    if (misaligned(t[i].param, p_item - 1) || misaligned(t[i].param_out, p_item - 1) || misaligned(t[i].grad, g_item - 1))
+      return fail(B200TP_ERR_OPTIM_INPUT, "a tensor is not aligned to its elements");
+    if (t[i].state_offset < 0 || t[i].state_offset % kBlock != 0)
+      return fail(B200TP_ERR_OPTIM_INPUT, "a tensor's place in the states must be a multiple of 256 elements");
+    const uintptr_t p = reinterpret_cast<uintptr_t>(t[i].param_out);
+    written.emplace_back(p, p + static_cast<uintptr_t>(t[i].numel) * p_item);
+    offsets.emplace_back(t[i].state_offset, t[i].state_offset + align_up(t[i].numel, kBlock));
+  }
+  const int rc = check_apart(written, "parameters");
+  return rc ? rc : check_apart(offsets, "states");
+}
+
+}  // namespace
+}  // namespace b200tp
+
+using namespace b200tp;
+
+extern "C" int b200tp_adamw_step(const b200tp_adamw_args* a, const b200tp_adamw_tensor* tensors, int32_t count, void* stream_v) {
+  try {
+    int rc = check(a, tensors, count);
+    if (rc) return rc;
+    if (count == 0) return B200TP_OK;
+    rc = require_sm100();
+    if (rc) return rc;
+    Rule r;
+    r.beta1 = static_cast<float>(a->beta1);
+    r.beta2 = static_cast<float>(a->beta2);
+    r.one_beta1 = static_cast<float>(1. - a->beta1);
+    r.one_beta2 = static_cast<float>(1. - a->beta2);
+    r.root_beta2 = static_cast<float>(std::sqrt(a->beta2));
+    r.root_one_beta2 = static_cast<float>(std::sqrt(1. - a->beta2));
+    r.eps = static_cast<float>(a->eps);
+    r.decay = static_cast<float>(1. - a->lr * a->weight_decay);
+    r.rate = static_cast<float>(a->lr / (1. - std::pow(a->beta1, static_cast<double>(a->step))));
+    r.root = static_cast<float>(1. / std::sqrt(1. - std::pow(a->beta2, static_cast<double>(a->step))));
+    r.grad_scale = static_cast<float>(a->grad_scale);
+    r.grad_scale_ptr = a->grad_scale_ptr;
+    r.step = static_cast<unsigned>(a->step);
+    States st;
+    st.m = a->exp_avg;
+    st.v = a->exp_avg_sq;
+    st.scales = static_cast<const float2*>(a->scales);
+    st.master = a->master;
+    st.m_out = a->exp_avg_out;
+    st.v_out = a->exp_avg_sq_out;
+    st.scales_out = static_cast<float2*>(a->scales_out);
+    st.master_out = a->master_out;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+    if (a->param_dtype == B200TP_BF16)
+      return a->grad_dtype == B200TP_BF16 ? launch_kind<__nv_bfloat16, __nv_bfloat16>(a, tensors, count, st, r, stream)
+                                          : launch_kind<__nv_bfloat16, float>(a, tensors, count, st, r, stream);
+    return a->grad_dtype == B200TP_BF16 ? launch_kind<float, __nv_bfloat16>(a, tensors, count, st, r, stream)
+                                        : launch_kind<float, float>(a, tensors, count, st, r, stream);
+  } catch (const std::exception& e) {
+    return fail(B200TP_ERR_OPTIM_INPUT, std::string("adamw: ") + e.what());
+  }
+}

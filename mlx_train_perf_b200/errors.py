@@ -29,6 +29,10 @@ class AttentionInputError(MlxTrainPerfError):
     """Shape validation failure at the flash_attention boundary."""
 
 
+class OptimizerInputError(MlxTrainPerfError):
+    """Shape/dtype/layout validation failure at the optimizer boundary."""
+
+
 class PackingError(MlxTrainPerfError):
     """Sequence-packing input validation failure."""
 

@@ -1,0 +1,398 @@
+"""The AdamW step against its definition in 64 bits, the layout of its states, and the optimizer around it.
+
+Tolerances count roundings of 2^-24 (half a step of fp32).  m: two factors rounded to fp32 (b1, 1 - b1), a product and a fused sum: 4 of
+|b1 m| + |c1 g|; v: 5 of b2 v + c2 g^2.  The update lr/bc1 m / (sqrt(v) bc2 + eps): what m is off by over the denominator, and
+4 (v under the root: half of 5, the root 2 with its Newton step) + 2 (bc2, eps) + 4 (reciprocal or quotient: 2 ulps) + 3 (rate, products)
+of its own, rounded up to 16.  p: 3 of |p| (decay, product, sum).  A stored bf16 value is off by another 2^-8.
+8-bit: a stored m is half an e4m3 step off (2^-4 of the value, or 2^-10 scales below 2^-6), a stored root one step at most.
+"""
+import copy
+import math
+
+import pytest
+import torch
+
+from mlx_train_perf_b200 import AdamW, AdamWState, OptimizerInputError, adamw_step
+
+pytestmark = pytest.mark.gpu
+
+E32 = 2.0 ** -24
+RULE = dict(lr=3e-3, betas=(0.9, 0.99), eps=1e-6, weight_decay=0.05)
+
+
+def _tensors(shapes, dtype, dev, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return [(torch.randn(s, generator=g) * scale).to(dtype).to(dev) for s in shapes]
+
+
+def _fill(state, seed):
+    """Moments in the middle of a run, by steps on random gradients."""
+    g = torch.Generator(device=state.exp_avg.device).manual_seed(seed)
+    dev = state.exp_avg.device
+    for t in range(3):
+        params = [torch.zeros(n, device=dev) for n in state.numels]
+        grads = [torch.randn(n, generator=g, device=dev) * 0.1 for n in state.numels]
+        master, state.master = state.master, None
+        adamw_step(params, grads, state, lr=0.0, betas=(0.9, 0.99))
+        state.master = master
+
+
+def _ref(p, g, m, v, step, grad_scale=1.0, *, lr, betas, eps, weight_decay):
+    """New p, m, v in 64 bits, and how far each may be off."""
+    p, g, m, v = p.double().reshape(-1), g.double().reshape(-1) * grad_scale, m.double(), v.double()
+    b1, b2 = betas
+    m1, v1 = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g * g
+    tm, tv = 4 * E32 * (b1 * m.abs() + (1 - b1) * g.abs()), 5 * E32 * v1
+    denom = (v1 / (1 - b2 ** step)).sqrt() + eps
+    rate = lr / (1 - b1 ** step)
+    p1 = p * (1 - lr * weight_decay) - rate * m1 / denom
+    tp = rate * tm / denom + 16 * E32 * (rate * m1 / denom).abs() + 3 * E32 * p.abs()
+    return p1, m1, v1, tp, tm, tv
+
+
+def _assert_within(got, want, tol, store=0.0):
+    off = (got.double().reshape(-1) - want).abs() - tol - store * want.abs() - 1e-37
+    assert not torch.isnan(got.float()).any() and (off.max().item() if off.numel() else 0.0) <= 0.0, off.max().item()
+
+
+def _e4m3_step(y):
+    """Distance of the e4m3 values around y."""
+    return 2.0 ** (torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -6))) - 3)
+
+
+def _check_moments(state, i, m1, v1, tm, tv):
+    m, v = state.moments(i)
+    if state.bits == 32:
+        _assert_within(m, m1, tm)
+        _assert_within(v, v1, tv)
+        return
+    scales = state.view("scales", i).double().repeat_interleave(256, 0)[:m.numel()]
+    zero = torch.zeros(m.numel(), dtype=torch.float64, device=m.device)
+    sm, sr = scales[:, 0], scales[:, 1]
+    _assert_within(m, m1, torch.where(sm > 0, 0.5 * _e4m3_step(m1 / sm.clamp(min=1e-300)) * sm, zero) * (1 + 64 * E32) + 2 * tm + 1e-29)
+    r1 = v1.sqrt()
+    step = torch.where(sr > 0, _e4m3_step(r1 / sr.clamp(min=1e-300)) * sr, zero)
+    _assert_within(v.sqrt(), r1, step * (1 + 64 * E32) + 16 * E32 * r1)
+    # a block's scales: its largest values over 448 (codes of the largest values are 448, or 416 where a dither went down)
+    n, blocks = m.numel(), state.view("scales", i)
+    pad = torch.zeros(blocks.shape[0] * 256, dtype=torch.float64, device=m.device)
+    for col, x in ((0, m1.abs()), (1, r1)):
+        pad.zero_()[:n] = x
+        torch.testing.assert_close(blocks[:, col].double(), pad.reshape(-1, 256).amax(1) / 448, rtol=32 * E32, atol=1e-32)
+    assert ((v > 0) == (v1 > 1e-30)).all()
+
+
+SHAPES = [(1,), (255,), (256,), (257,), (3, 5, 7), (4096,), (0,), (64, 129), (20011,)]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("p_dtype,g_dtype,master", [(torch.float32, torch.float32, False), (torch.float32, torch.bfloat16, False),
+                                                    (torch.bfloat16, torch.bfloat16, False), (torch.bfloat16, torch.float32, False),
+                                                    (torch.bfloat16, torch.bfloat16, True), (torch.bfloat16, torch.float32, True)])
+@pytest.mark.parametrize("scale", [1.0, 0.125])
+def test_step(cuda_device, bits, p_dtype, g_dtype, master, scale):
+    dev = cuda_device
+    params, grads = _tensors(SHAPES, p_dtype, dev, 1), _tensors(SHAPES, g_dtype, dev, 2, 0.2)
+    state = AdamWState.zeros(params, bits=bits, master=master)
+    _fill(state, 5)
+    before = [tuple(t.clone() for t in state.moments(i)) for i in range(len(SHAPES))]
+    values = [(state.view("master", i) if master else p.reshape(-1)).clone() for i, p in enumerate(params)]
+    assert state.steps == [3] * len(SHAPES)
+    how = torch.tensor([scale], device=dev) if scale != 1.0 else 1.0
+    adamw_step(params, grads, state, grad_scale=how, **RULE)
+    assert state.steps == [4] * len(SHAPES)
+    for i, (p, g) in enumerate(zip(params, grads)):
+        p1, m1, v1, tp, tm, tv = _ref(values[i], g, *before[i], 4, scale, **RULE)
+        _assert_within(p, p1, tp, 2.0 ** -8 * (1 + 2.0 ** -16) if p_dtype == torch.bfloat16 else 0.0)
+        if master:
+            _assert_within(state.view("master", i), p1, tp)
+            assert torch.equal(p.reshape(-1), state.view("master", i).to(torch.bfloat16))
+        _check_moments(state, i, m1, v1, tm, tv)
+    # what lies behind each tensor in the states stays zero
+    for name in ("exp_avg", "exp_avg_sq") + (("master",) if master else ()):
+        flat = getattr(state, name).float()
+        for i in range(len(SHAPES)):
+            o, n = int(state.rows[i, 4]), state.numels[i]
+            assert (flat[o + n:o + (n + 255) // 256 * 256] == 0).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("master", [False, True])
+def test_other_buffers_get_what_the_step_in_place_gives(cuda_device, bits, master):
+    dev = cuda_device
+    params, grads = _tensors(SHAPES, torch.bfloat16, dev, 3), _tensors(SHAPES, torch.bfloat16, dev, 4)
+    state = AdamWState.zeros(params, bits=bits, master=master)
+    _fill(state, 6)
+    names = [n for n in ("exp_avg", "exp_avg_sq", "scales", "master") if getattr(state, n) is not None]
+    kept = {n: getattr(state, n).clone() for n in names}
+    old = [p.clone() for p in params]
+    to = [torch.full_like(p, float("nan")) for p in params]
+    after = AdamWState.zeros(params, bits=bits, master=master)
+    adamw_step(params, grads, state, step=9, out=(to, after), **RULE)
+    assert all(torch.equal(p, q) for p, q in zip(params, old)) and state.steps == [3] * len(SHAPES) and after.steps == [9] * len(SHAPES)
+    assert all(torch.equal(getattr(state, n).view(torch.uint8), kept[n].view(torch.uint8)) for n in names)
+    adamw_step(params, grads, state, step=9, **RULE)
+    assert all(torch.equal(p, q) for p, q in zip(params, to))
+    assert all(torch.equal(getattr(state, n).view(torch.uint8), getattr(after, n).view(torch.uint8)) for n in names)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_unaligned_views_and_strided_gradients(cuda_device, bits):
+    """Parameters and gradients one element off an aligned address, odd sizes, gradients transposed: the values of aligned ones."""
+    dev = cuda_device
+    sizes = [(3, 301), (17, 1000), (4099,)]
+    got = []
+    for off in (0, 1):
+        params = [torch.empty(math.prod(s) + 8, dtype=torch.bfloat16, device=dev)[off:off + math.prod(s)].view(s).copy_(t)
+                  for s, t in zip(sizes, _tensors(sizes, torch.bfloat16, dev, 7))]
+        grads = [torch.empty(math.prod(s) + 8, dtype=torch.bfloat16, device=dev)[off:off + math.prod(s)].view(s).copy_(t)
+                 for s, t in zip(sizes, _tensors(sizes, torch.bfloat16, dev, 8))]
+        if off:
+            grads[0] = grads[0].t().contiguous().t()
+        around = [p._base[-8 + off:].clone() for p in params]
+        state = AdamWState.zeros(params, bits=bits)
+        adamw_step(params, grads, state, **RULE)
+        adamw_step(params, grads, state, **RULE)
+        assert all(torch.equal(p._base[-8 + off:].view(torch.int16), a.view(torch.int16)) for p, a in zip(params, around))
+        got.append([*(p.clone() for p in params), state.exp_avg.view(torch.uint8), state.exp_avg_sq.view(torch.uint8)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_more_tensors_than_one_launch_takes(cuda_device):
+    dev = cuda_device
+    for count in (48, 49, 600, 601, 1300):
+        params = [torch.full((1 + k % 3,), float(k), device=dev) for k in range(count)]
+        grads = [torch.full((1 + k % 3,), 0.5 - k % 2, device=dev) for k in range(count)]
+        state = AdamWState.zeros(params)
+        adamw_step(params, grads, state, lr=0.25, weight_decay=0.0, eps=0.0)
+        for k, p in enumerate(params):            # the first step moves by lr against the gradient's sign
+            assert (p - (k + (0.25 if k % 2 else -0.25))).abs().max().item() <= 4e-7 * max(1, k), k
+
+
+def test_tensors_without_gradients_and_of_different_ages(cuda_device):
+    dev = cuda_device
+    shapes = [(300,), (5,), (1000,)]
+    params, grads = _tensors(shapes, torch.float32, dev, 9), _tensors(shapes, torch.float32, dev, 10)
+    state = AdamWState.zeros(params)
+    alone = [AdamWState.zeros([p]) for p in params]
+    single = [p.clone() for p in params]
+    for which in ((0, 1, 2), (0, 2), (1,), (), (0, 1, 2)):
+        adamw_step(params, [g if i in which else None for i, g in enumerate(grads)], state, **RULE)
+        for i in which:
+            adamw_step([single[i]], [grads[i]], alone[i], **RULE)
+    assert state.steps == [3, 3, 3] and all(torch.equal(p, q) for p, q in zip(params, single))
+    adamw_step(params, [grads[0], None, None], state, **RULE)
+    assert state.steps == [4, 3, 3]
+    adamw_step(params, grads, state, **RULE)                      # two ages in one call
+    for i in ([0, 0], [1], [2]):
+        for k in i:
+            adamw_step([single[k]], [grads[k]], alone[k], **RULE)
+    assert state.steps == [5, 4, 4] and all(torch.equal(p, q) for p, q in zip(params, single))
+
+
+def test_8_bit_roots_are_rounded_without_drift(cuda_device):
+    """A million equal roots between two codes: the mean of the codes is the root, up to five standard errors and the dither's own
+    2^-17 of a step; and a v that is not zero never becomes zero, whatever the block's largest."""
+    dev = cuda_device
+    n = 1 << 20
+    p = [torch.zeros(n, device=dev)]
+    g = torch.full((n,), 1.3, device=dev)
+    g[::256] = 7.0                                                # the blocks' scale
+    state = AdamWState.zeros(p, bits=8)
+    adamw_step(p, [g], state, lr=0.0, betas=(0.0, 0.0))
+    roots = state.moments(0)[1].sqrt().double().reshape(-1, 256)[:, 1:]
+    step = 2.0 ** (math.floor(math.log2(1.3 / (7.0 / 448))) - 3) * 7.0 / 448
+    se = step / 2 / math.sqrt(roots.numel())
+    assert roots.unique().numel() == 2 and abs(roots.mean().item() - 1.3) < 5 * se + step * 2.0 ** -17 + 1.3 * 8 * E32
+    # the same step again gives the same codes, the next one others
+    again = AdamWState.zeros(p, bits=8)
+    adamw_step(p, [g], again, lr=0.0, betas=(0.0, 0.0))
+    assert torch.equal(again.exp_avg_sq.view(torch.uint8), state.exp_avg_sq.view(torch.uint8))
+    adamw_step(p, [g], again, lr=0.0, betas=(0.0, 0.0))
+    assert not torch.equal(again.exp_avg_sq.view(torch.uint8), state.exp_avg_sq.view(torch.uint8))
+    g = torch.full((n,), 1e-12, device=dev)
+    g[::256] = 1e6
+    g[1::256] = 0.0
+    adamw_step(p, [g], state, lr=0.0, betas=(0.0, 0.0))
+    v = state.moments(0)[1].reshape(-1, 256)
+    assert (v[:, 1] == 0).all() and (v[:, 2:] > 0).all() and (v[:, 0] > 0).all()
+
+
+def test_8_bit_moments_follow_a_falling_gradient(cuda_device):
+    """Gradients of one element fall to zero while its block's largest stays: rounding to nearest would hold its root for ever
+    (a step changes it by 0.05 %, half a code's distance is 3 %); after 3000 steps with b2 = 0.999 it has shrunk to exp(-1.5)
+    = 0.22 of itself, give or take the walk's deviation of some 25 %."""
+    dev = cuda_device
+    n = 256 * 64
+    p, state = [torch.zeros(n, device=dev)], AdamWState.zeros([torch.zeros(n, device=dev)], bits=8)
+    hot = torch.zeros(n, device=dev)
+    hot[::256] = 4.0
+    adamw_step(p, [torch.ones(n, device=dev) + hot], state, lr=0.0, betas=(0.9, 0.0))
+    for _ in range(3000):
+        adamw_step(p, [hot + (hot > 0)], state, lr=0.0, betas=(0.9, 0.999))
+    roots = state.moments(0)[1].sqrt().reshape(-1, 256)[:, 1:]
+    assert 0.17 < roots.double().square().mean().sqrt().item() < 0.3 and 0.17 < roots.mean().item() < 0.27
+
+
+def test_what_is_not_finite_stays_by_itself(cuda_device):
+    """8 bits: NaN, infinity and an overflowing square void their own element and no other of the block; 32 bits the same."""
+    dev = cuda_device
+    for bits in (8, 32):
+        g = torch.randn(1000, generator=torch.Generator().manual_seed(3)).to(dev)
+        clean = g.clone()
+        g[5], g[300], g[301], g[302] = math.nan, math.inf, -math.inf, 1e25
+        bad = torch.zeros(1000, dtype=torch.bool, device=dev)
+        bad[[5, 300, 301, 302]] = True
+        clean[bad] = 0.0
+        got = []
+        for t in (g, clean):
+            p = [torch.ones(1000, device=dev)]
+            state = AdamWState.zeros(p, bits=bits)
+            adamw_step(p, [t], state, **RULE)
+            adamw_step(p, [t.nan_to_num(0.0, 0.0, 0.0).clamp(-10, 10)], state, **RULE)
+            got.append((p[0], *state.moments(0)))
+        for a, b in zip(*got):
+            assert torch.equal(a[~bad], b[~bad])
+        assert torch.isnan(got[0][1][[5, 300, 301]]).logical_or(torch.isinf(got[0][1][[5, 300, 301]])).all()
+        assert not torch.isfinite(got[0][2][bad]).any()
+
+
+def test_tensors_that_share_memory_are_refused(cuda_device):
+    dev = cuda_device
+    p = torch.zeros(1000, device=dev)
+    g = torch.zeros(1000, device=dev)
+    for pair in ([p, p], [p[:600], p[400:]]):
+        state = AdamWState.zeros(pair)
+        with pytest.raises(OptimizerInputError, match="share memory"):
+            adamw_step(pair, [g[:t.numel()] for t in pair], state, **RULE)
+    touching = [p[:500], p[500:]]
+    adamw_step(touching, [g[:500], g[500:]], AdamWState.zeros(touching), **RULE)
+
+
+def test_refusals(cuda_device):
+    dev = cuda_device
+    p, g = [torch.zeros(8, 4, device=dev)], [torch.zeros(8, 4, device=dev)]
+    s = AdamWState.zeros(p)
+    s8 = AdamWState.zeros(p, bits=8)
+    m32 = torch.zeros(256, device=dev)
+    bad = [
+        lambda: adamw_step(p, g + g, s, lr=0.1), lambda: adamw_step(p, [g[0].cpu()], s, lr=0.1), lambda: adamw_step(p, [g[0].half()], s, lr=0.1),
+        lambda: adamw_step(p, [g[0][:4]], s, lr=0.1), lambda: adamw_step([p[0].t()], g, s, lr=0.1), lambda: adamw_step([p[0].double()], g, s, lr=0.1),
+        lambda: adamw_step([p[0].cpu()], g, s, lr=0.1), lambda: adamw_step(p, g, s, lr=-0.1), lambda: adamw_step(p, g, s, lr=0.1, betas=(1.0, 0.9)),
+        lambda: adamw_step(p, g, s, lr=0.1, betas=(0.9, -0.1)), lambda: adamw_step(p, g, s, lr=0.1, eps=-1.0), lambda: adamw_step(p, g, s, lr=0.1, weight_decay=-1.0),
+        lambda: adamw_step(p, g, s, lr=0.1, step=0), lambda: adamw_step(p, [None], s, lr=0.1, out=(p, s)), lambda: adamw_step(p, g, s, lr=0.1, out=(p, s8)),
+        lambda: adamw_step(p, g, s, lr=0.1, grad_scale=torch.ones(2, device=dev)), lambda: adamw_step(p, g, s, lr=0.1, grad_scale=torch.ones(1)),
+        lambda: adamw_step(p, [g[0].to_sparse()], s, lr=0.1), lambda: adamw_step(p, g, s, lr=float("nan")),
+        lambda: AdamWState.zeros(p, bits=16), lambda: AdamWState.zeros([]), lambda: AdamWState.zeros([p[0].cpu()]),
+        lambda: AdamWState([32], m32[:128], m32), lambda: AdamWState([32], m32, m32.cpu()), lambda: AdamWState([32], m32, m32, scales=torch.zeros(1, 2, device=dev)),
+        lambda: AdamWState([32], m32, m32, steps=[1, 2]), lambda: adamw_step(p, g, AdamWState.zeros(p, master=True), lr=0.1),
+        lambda: adamw_step(p, g, AdamWState([32], torch.zeros(260, device=dev)[1:257], m32), lr=0.1),
+        lambda: AdamW(p, bits=4),
+    ]
+    for k, call in enumerate(bad):
+        with pytest.raises(OptimizerInputError):
+            call()
+            pytest.fail(f"call {k} was not refused")
+    assert s.steps == [0] and (p[0] == 0).all()
+
+
+def _model(dev, dtype=torch.float32, seed=0):
+    torch.manual_seed(seed)
+    return torch.nn.Sequential(torch.nn.Linear(33, 70), torch.nn.Tanh(), torch.nn.Linear(70, 9)).to(dev).to(dtype)
+
+
+def _train(model, opt, steps, seed=1, scheduler=None):
+    g = torch.Generator().manual_seed(seed)
+    p = next(model.parameters())
+    for _ in range(steps):
+        x = torch.randn(16, 33, generator=g).to(p.device).to(p.dtype)
+        opt.zero_grad(set_to_none=True)
+        model(x).float().square().mean().backward()
+        opt.step()
+        if scheduler is not None:
+            scheduler.step()
+
+
+def test_optimizer_against_torch(cuda_device):
+    """Ten steps with two groups and a schedule beside torch's AdamW in fp64.  Each step is within 16 x 2^-24 of its length, but
+    gradients feed back; 1e-5 of the largest weight is some hundred of those."""
+    a, b = _model(cuda_device), _model(cuda_device, torch.float64)
+    groups = lambda m: [{"params": m[0].parameters()}, {"params": m[2].parameters(), "lr": 3e-3, "weight_decay": 0.2}]
+    ours, theirs = AdamW(groups(a), lr=1e-2), torch.optim.AdamW(groups(b), lr=1e-2)
+    _train(a, ours, 10, scheduler=torch.optim.lr_scheduler.ExponentialLR(ours, 0.8))
+    _train(b, theirs, 10, scheduler=torch.optim.lr_scheduler.ExponentialLR(theirs, 0.8))
+    for p, q in zip(a.parameters(), b.parameters()):
+        assert (p.double() - q).abs().max() < 1e-5 * q.abs().max()
+
+
+@pytest.mark.parametrize("bits,master", [(32, False), (8, True)])
+def test_saved_and_loaded_optimizer_goes_on_alike(cuda_device, bits, master):
+    import io
+    dtype = torch.bfloat16 if master else torch.float32
+    a = _model(cuda_device, dtype)
+    opt = AdamW(a.parameters(), lr=1e-2, bits=bits, master=master)
+    _train(a, opt, 4)
+    buffer = io.BytesIO()
+    torch.save({"model": a.state_dict(), "opt": opt.state_dict()}, buffer)
+    buffer.seek(0)
+    saved = torch.load(buffer)
+    b = _model(cuda_device, dtype, seed=5)
+    b.load_state_dict(saved["model"])
+    other = AdamW(b.parameters(), lr=1.0, bits=bits, master=master)
+    other.load_state_dict(saved["opt"])
+    third, c = copy.deepcopy((opt, a))                            # one deep copy of both: the copy's groups hold the copied parameters
+    for m, o in ((a, opt), (b, other), (c, third)):
+        _train(m, o, 3, seed=2)
+    for p, q, r in zip(a.parameters(), b.parameters(), c.parameters()):
+        assert torch.equal(p, q) and torch.equal(p, r)
+    one, two = opt.state_dict(), other.state_dict()
+    assert one["param_groups"] == two["param_groups"] and all(s["step"] == 7 for s in one["state"].values())
+    for k in one["state"]:
+        for name, t in one["state"][k].items():
+            if name != "step":
+                assert torch.equal(t.view(torch.uint8), two["state"][k][name].view(torch.uint8))
+    with pytest.raises(OptimizerInputError):
+        AdamW(b.parameters(), bits=40 - bits, master=master).load_state_dict(saved["opt"])
+
+
+def test_mixed_dtypes_missing_gradients_and_versions(cuda_device):
+    dev = cuda_device
+    p = [torch.nn.Parameter(t) for t in (torch.ones(10, device=dev), torch.ones(300, device=dev, dtype=torch.bfloat16), torch.ones(7, device=dev))]
+    opt = AdamW(p, lr=0.5, weight_decay=0.0, master=True)
+    opt.step()                                                    # nothing to do
+    p[0].grad, p[1].grad = torch.ones_like(p[0]), -torch.ones_like(p[1])
+    y = (p[0] * p[0]).sum()                                       # keeps p[0] for its backward
+    version = p[0]._version
+    opt.step()
+    assert (p[0] == 0.5).all() and (p[1] == 1.5).all() and (p[2] == 1.0).all() and p[0]._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_capture_is_refused_and_other_streams_work(cuda_device):
+    dev = cuda_device
+    p = torch.nn.Parameter(torch.ones(5000, device=dev))
+    opt = AdamW([p], lr=0.5, weight_decay=0.0)
+    p.grad = torch.ones_like(p)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert (p == 0.5).all()
+    refused, graph, one = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph(), torch.ones(1, device=dev)
+    with pytest.raises(OptimizerInputError, match="captured"):
+        with torch.cuda.graph(refused):
+            one.add_(1)
+            opt.step()
+    torch.cuda.synchronize()
+    # the step on lists with its number given can be captured; a replay repeats that very step
+    state = AdamWState.zeros([p])
+    to, after = [torch.empty_like(p)], AdamWState.zeros([p])
+    with torch.cuda.graph(graph):
+        adamw_step([p.detach()], [p.grad], state, lr=0.25, weight_decay=0.0, step=1, out=(to, after))
+    for g in (1.0, -1.0):
+        p.grad.fill_(g)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (to[0] - (0.5 - 0.25 * g)).abs().max() < 1e-6

@@ -1,0 +1,110 @@
+"""Refusals of the objectives' and the optimizer's C entry points, which come before anything is launched (no GPU needed), and the
+Python checks that host tensors reach."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from mlx_train_perf_b200 import AdamW, AdamWState, LossInputError, OptimizerInputError, _lib, policy_loss, preference_loss
+from mlx_train_perf_b200.build import build
+
+PTR = 1 << 20                          # a non-null placeholder: nothing is dereferenced
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build(verbose=False)
+    return _lib.load()
+
+
+def _objective(**change):
+    a = _lib.ObjectiveArgs(PTR, PTR, PTR, None, PTR, None, 4, 100, 100, 100, 100, 0, 1, 0, 0, 0, 0, 0)
+    for k, v in change.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("change,text", [
+    ({"seqs": 0}, b"number of sequences"), ({"seqs": 1 << 30}, b"number of sequences"), ({"length": -1}, b"negative length"),
+    ({"length": 1 << 40}, b"2^30"), ({"dtype": 7}, b"fp32 or bf16"), ({"other_dtype": 2}, b"fp32 or bf16"), ({"logps": None}, b"logps is null")])
+def test_objective_arguments(lib, change, text):
+    a = _objective(**change)
+    assert lib.b200tp_objective_workspace_bytes(C.byref(a)) == 0
+    assert text in lib.b200tp_last_error()
+    assert lib.b200tp_preference_loss_fwd(C.byref(a), 0, 0.1, 0.0, 0.0, 0, PTR, PTR, PTR, PTR, 1 << 20, None) == _lib.ERR_LOSS_INPUT
+    assert lib.b200tp_policy_loss_fwd(C.byref(a), 0.2, 0.2, 0.0, 2, 0, PTR, PTR, PTR, PTR, 1 << 20, None) == _lib.ERR_LOSS_INPUT
+    assert lib.b200tp_objective_bwd(C.byref(a), None, PTR, 1, PTR, PTR, None) == _lib.ERR_LOSS_INPUT
+
+
+def test_objective_rules_and_workspace(lib):
+    a = _objective()
+    need = lib.b200tp_objective_workspace_bytes(C.byref(a))
+    assert 0 < need <= 4096 and need % 256 == 0
+    pref = lambda a, kind=0, beta=0.1, loss=PTR, ws=PTR, n=need: lib.b200tp_preference_loss_fwd(
+        C.byref(a), kind, beta, 0.0, 0.0, 0, loss, PTR, PTR, ws, n, None)
+    assert pref(_objective(seqs=3)) == _lib.ERR_LOSS_INPUT and pref(a, kind=3) == _lib.ERR_LOSS_INPUT
+    assert pref(a, beta=0.0) == _lib.ERR_LOSS_INPUT and pref(a, beta=float("nan")) == _lib.ERR_LOSS_INPUT and pref(a, loss=None) == _lib.ERR_LOSS_INPUT
+    assert pref(a, ws=None) == _lib.ERR_WORKSPACE and pref(a, ws=PTR + 8) == _lib.ERR_WORKSPACE and pref(a, n=need - 1) == _lib.ERR_WORKSPACE
+    pol = lambda a, low=0.2, high=0.2, coef=0.1, kl=2, norm=0: lib.b200tp_policy_loss_fwd(
+        C.byref(a), low, high, coef, kl, norm, PTR, PTR, PTR, PTR, need, None)
+    for bad in (dict(low=-0.1), dict(low=1.1), dict(high=-1.0), dict(kl=3), dict(norm=3), dict(norm=-1), dict(low=float("nan"))):
+        assert pol(a, **bad) == _lib.ERR_LOSS_INPUT, bad
+    assert pol(_objective(ref_logps=None)) == _lib.ERR_LOSS_INPUT and b"KL term" in lib.b200tp_last_error()
+    assert pol(_objective(old_logps=None)) == _lib.ERR_LOSS_INPUT and pol(_objective(advantages=None)) == _lib.ERR_LOSS_INPUT
+    assert lib.b200tp_objective_bwd(C.byref(a), PTR, None, 1, PTR, PTR, None) == _lib.ERR_LOSS_INPUT
+
+
+def test_workspace_grows_with_sequences_not_tokens(lib):
+    """Sums of 32 bytes for each block: at most 512 blocks a sequence and about eight an SM in all."""
+    for seqs, length in ((1, 1 << 30), (2, 1 << 20), (512, 8192), (1 << 20, 4)):
+        a = _objective(seqs=seqs, length=length)
+        assert 32 * seqs <= lib.b200tp_objective_workspace_bytes(C.byref(a)) <= 32 * max(seqs, 2 * 1184) + 256
+
+
+def _adamw(rows, **change):
+    a = _lib.AdamwArgs(PTR, PTR, None, None, PTR, PTR, None, None, 1e-3, 0.9, 0.999, 1e-8, 0.01, 1.0, None, 1, 0, 0, 32, 0)
+    for k, v in change.items():
+        setattr(a, k, v)
+    rows = np.array(rows, dtype=np.int64).reshape(-1, 5)
+    return _lib.load().b200tp_adamw_step(C.byref(a), rows.ctypes.data, len(rows), None)
+
+
+ROW = [PTR, PTR, PTR, 100, 0]
+
+
+@pytest.mark.parametrize("change", [dict(bits=16), dict(param_dtype=3), dict(grad_dtype=2), dict(step=0), dict(beta1=1.0), dict(beta2=-0.1),
+                                    dict(eps=-1.0), dict(lr=-1.0), dict(lr=float("nan")), dict(weight_decay=-0.1), dict(exp_avg=None), dict(exp_avg_sq_out=None),
+                                    dict(bits=8), dict(master=PTR), dict(master=PTR, master_out=PTR), dict(exp_avg=PTR + 4), dict(exp_avg_out=PTR + 8)])
+def test_adamw_arguments(lib, change):
+    assert _adamw([ROW], **change) == _lib.ERR_OPTIM_INPUT
+
+
+@pytest.mark.parametrize("rows", [
+    [[0, PTR, PTR, 100, 0]], [[PTR, 0, PTR, 100, 0]], [[PTR, PTR, 0, 100, 0]], [[PTR, PTR, PTR, -1, 0]], [[PTR, PTR, PTR, 100, 128]],
+    [[PTR, PTR, PTR, 100, -256]], [[PTR + 1, PTR, PTR, 100, 0]], [[PTR, PTR + 2, PTR, 100, 0]],
+    [ROW, ROW], [ROW, [PTR, PTR, PTR + 396, 100, 256]], [ROW, [PTR, PTR, PTR + 400, 100, 0]], [[PTR, PTR, PTR, 257, 0], [PTR, PTR, PTR + 4096, 8, 256]]])
+def test_adamw_tables(lib, rows):
+    assert _adamw(rows) == _lib.ERR_OPTIM_INPUT
+
+
+def test_adamw_of_nothing(lib):
+    assert _adamw([]) == _lib.OK
+
+
+def test_status_text(lib):
+    assert lib.b200tp_status_string(_lib.ERR_OPTIM_INPUT) == b"optimizer input error"
+
+
+def test_host_tensors_are_refused():
+    x, a = torch.zeros(2, 4), torch.zeros(2, 1)
+    with pytest.raises(LossInputError, match="CUDA"):
+        preference_loss(x)
+    with pytest.raises(LossInputError, match="CUDA"):
+        policy_loss(x, x, a)
+    with pytest.raises(OptimizerInputError, match="CUDA"):
+        AdamWState.zeros([x])
+    p = torch.nn.Parameter(x)
+    p.grad = torch.zeros_like(x)
+    with pytest.raises(OptimizerInputError, match="CUDA"):
+        AdamW([p]).step()
