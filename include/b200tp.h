@@ -39,12 +39,14 @@ extern "C" {
 #define B200TP_ERR_CUDA 6              /* a CUDA runtime / driver call failed */
 #define B200TP_ERR_NO_DEVICE 7         /* current device is not compute capability 10.x */
 #define B200TP_ERR_OPTIM_INPUT 8       /* maps to OptimizerInputError */
+#define B200TP_ERR_EMBEDDING_INPUT 9   /* maps to EmbeddingInputError */
 
 /* device-side status words (written into `status`) */
 #define B200TP_DEV_TIMEOUT_PRODUCER 101
 #define B200TP_DEV_TIMEOUT_MMA 102
 #define B200TP_DEV_TIMEOUT_EPILOGUE 103
 #define B200TP_DEV_TIMEOUT_OTHER 104
+#define B200TP_DEV_BAD_INDEX 105       /* no wait: an embedding id outside the table */
 
 /* implementation selectors */
 #define B200TP_IMPL_AUTO 0   /* tcgen05 path for bf16 (head_dim 128 for attention), SIMT otherwise */
@@ -421,6 +423,31 @@ typedef struct b200tp_adamw_args {
  * fp32, each stored value rounded once.  `tensors` is host memory, read before the call returns; up to 600 tensors a
  * launch.  Tensors that share memory are refused. */
 int b200tp_adamw_step(const b200tp_adamw_args* a, const b200tp_adamw_tensor* tensors, int32_t count, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Embedding lookup
+ * ------------------------------------------------------------------------------------- */
+
+typedef struct b200tp_embedding_args {
+  const void* ids;       /* (n,) int32 or int64; one outside [0, v) gives a row of zeros, no gradient and *status */
+  int64_t n, v;          /* tokens, rows of the table */
+  int32_t d;             /* columns */
+  int32_t dtype;         /* of table, output and both gradients */
+  int32_t ids_int64;
+  float scale;
+  int64_t row_stride;    /* elements between rows of the table (fwd) or of d_out (bwd); columns are adjacent */
+  int64_t padding_idx;   /* an id whose row gets no gradient (it is looked up like any other), or -1 */
+} b200tp_embedding_args;
+
+/* out (n, d) contiguous: out[i] = scale * weight[ids[i]], rounded once.  The reference calls its model's own embedding
+ * (adapters/mlx_lm.py:140-164). */
+int b200tp_embedding_fwd(const b200tp_embedding_args* a, const void* weight, void* out, void* stream, int* status);
+
+/* d_weight (v, d) contiguous, 16-byte aligned, every row written: scale times the sum, in the order of i and in f32, of d_out[i] over the
+ * tokens with that id. */
+size_t b200tp_embedding_bwd_workspace_bytes(const b200tp_embedding_args* a);
+int b200tp_embedding_bwd(const b200tp_embedding_args* a, const void* d_out, void* d_weight, void* workspace,
+                         size_t workspace_bytes, void* stream, int* status);
 
 #ifdef __cplusplus
 }

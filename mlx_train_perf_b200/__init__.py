@@ -2,13 +2,13 @@
 
 Public surface (mirrors src/mlx_train_perf/__init__.py and the modules it re-exports):
 `linear_cross_entropy`, `fused_linear_ce`, `DenseHead`, `QuantizedHead`, `tied_head`,
-`preference_loss`, `policy_loss`, `flash_attention`, `PackedMask`, `enable_flash_attention`, `packed_iterate_batches`,
-`plan_fit`.  Every numeric operator is a thin ctypes wrapper over one C-ABI CUDA library
+`preference_loss`, `policy_loss`, `embedding_lookup`, `AdamW`, `adamw_step`, `flash_attention`, `PackedMask`,
+`enable_flash_attention`, `packed_iterate_batches`, `plan_fit`.  Every numeric operator is a thin ctypes wrapper over one C-ABI CUDA library
 (`csrc/`), and raises `NativeLibraryError` when that library cannot be loaded.
 """
 from mlx_train_perf_b200.errors import (  # noqa: F401
-    AdapterError, AttentionInputError, DeviceTimeoutError, DoesNotFitError, LossInputError,
-    MlxTrainPerfError, NativeLibraryError, OptimizerInputError, PackingError, PlanInputError,
+    AdapterError, AttentionInputError, DeviceTimeoutError, DoesNotFitError, EmbeddingInputError,
+    LossInputError, MlxTrainPerfError, NativeLibraryError, OptimizerInputError, PackingError, PlanInputError,
     UnsupportedAttentionError, UnsupportedHeadError,
 )
 
@@ -22,6 +22,7 @@ _LAZY = {
     "tied_head": "mlx_train_perf_b200.core.loss",
     "preference_loss": "mlx_train_perf_b200.core.objectives",
     "policy_loss": "mlx_train_perf_b200.core.objectives",
+    "embedding_lookup": "mlx_train_perf_b200.core.embedding",
     "AdamW": "mlx_train_perf_b200.core.optim",
     "AdamWState": "mlx_train_perf_b200.core.optim",
     "adamw_step": "mlx_train_perf_b200.core.optim",

@@ -13,7 +13,7 @@ from pathlib import Path
 import torch
 
 from mlx_train_perf_b200.errors import (
-    AttentionInputError, DeviceTimeoutError, LossInputError, NativeLibraryError, OptimizerInputError,
+    AttentionInputError, DeviceTimeoutError, EmbeddingInputError, LossInputError, NativeLibraryError, OptimizerInputError,
     UnsupportedAttentionError, UnsupportedHeadError,
 )
 
@@ -25,7 +25,8 @@ IMPL = {"auto": 0, "kernel": 0, "tc": 1, "simt": 2}
 OK = 0
 ERR_LOSS_INPUT, ERR_UNSUPPORTED_HEAD, ERR_ATTN_INPUT, ERR_UNSUPPORTED_ATTN = 1, 2, 3, 4
 ERR_WORKSPACE, ERR_CUDA, ERR_NO_DEVICE = 5, 6, 7
-ERR_OPTIM_INPUT = 8
+ERR_OPTIM_INPUT, ERR_EMBEDDING_INPUT = 8, 9
+DEV_BAD_INDEX = 105
 
 
 class CeArgs(C.Structure):
@@ -80,6 +81,13 @@ class AdamwArgs(C.Structure):
         ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
         ("grad_scale", C.c_double), ("grad_scale_ptr", C.c_void_p), ("step", C.c_int64),
         ("param_dtype", C.c_int32), ("grad_dtype", C.c_int32), ("bits", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class EmbeddingArgs(C.Structure):
+    _fields_ = [
+        ("ids", C.c_void_p), ("n", C.c_int64), ("v", C.c_int64), ("d", C.c_int32), ("dtype", C.c_int32),
+        ("ids_int64", C.c_int32), ("scale", C.c_float), ("row_stride", C.c_int64), ("padding_idx", C.c_int64),
     ]
 
 
@@ -142,6 +150,10 @@ SIGNATURES = {
                                    C.c_size_t, C.c_void_p, C.c_void_p]),
     # the tensors: (count, 5) int64 rows param, grad, param_out, numel, state_offset
     "b200tp_adamw_step": (C.c_int, [C.POINTER(AdamwArgs), C.c_void_p, C.c_int32, C.c_void_p]),
+    "b200tp_embedding_fwd": (C.c_int, [C.POINTER(EmbeddingArgs), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "b200tp_embedding_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(EmbeddingArgs)]),
+    "b200tp_embedding_bwd": (C.c_int, [C.POINTER(EmbeddingArgs), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p,
+                                       C.c_void_p]),
     "b200tp_objective_workspace_bytes": (C.c_size_t, [C.POINTER(ObjectiveArgs)]),
     "b200tp_preference_loss_fwd": (C.c_int, [C.POINTER(ObjectiveArgs), C.c_int32, C.c_double, C.c_double, C.c_double,
                                              C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
@@ -204,6 +216,7 @@ _ERRORS = {
     ERR_ATTN_INPUT: AttentionInputError,
     ERR_UNSUPPORTED_ATTN: UnsupportedAttentionError,
     ERR_OPTIM_INPUT: OptimizerInputError,
+    ERR_EMBEDDING_INPUT: EmbeddingInputError,
     ERR_WORKSPACE: NativeLibraryError,
     ERR_CUDA: NativeLibraryError,
     ERR_NO_DEVICE: NativeLibraryError,
@@ -221,8 +234,10 @@ def check(rc: int) -> None:
 
 
 def raise_for_device_status(code: int) -> None:
-    """Raise `DeviceTimeoutError` for a non-zero device status word (read after a sync)."""
+    """Raise `DeviceTimeoutError` for a non-zero device status word (read after a sync), or what else the word names."""
     if code == 0:
         return
     name = (load().b200tp_status_string(code) or b"").decode()
+    if code == DEV_BAD_INDEX:
+        raise EmbeddingInputError(name)
     raise DeviceTimeoutError(f"kernel reported status {code}: {name}")

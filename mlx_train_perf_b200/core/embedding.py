@@ -1,0 +1,98 @@
+"""`embedding_lookup`: scaled rows of a table, and the table's gradient by sorted tokens (csrc/embedding.cu).
+
+The reference's trunk calls the model's own embedding module (adapters/mlx_lm.py:140-164); the adapters here use this
+operator where the table is trained.  The gradient adds the rows of equal ids in the order of the tokens, in fp32,
+rounds once, and is the same bits for equal calls.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from mlx_train_perf_b200 import _lib
+from mlx_train_perf_b200.core.loss import VJP_CALLS, device_status
+from mlx_train_perf_b200.errors import EmbeddingInputError
+
+_DTYPES = (torch.float32, torch.bfloat16)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """(N, D) with adjacent columns."""
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+class _Lookup(torch.autograd.Function):
+    """(weight, ids (N,), scale, padding) -> (N, D)."""
+
+    @staticmethod
+    def forward(ctx, weight, ids, scale, padding):
+        n, (v, d) = ids.shape[0], weight.shape
+        dev = weight.device
+        rows = _rows(weight)
+        out = torch.empty((n, d), dtype=weight.dtype, device=dev)
+        a = _lib.EmbeddingArgs(ids.data_ptr(), n, v, d, weight.dtype == torch.bfloat16, ids.dtype == torch.int64, scale, rows.stride(0),
+                               padding)
+        with _lib.on(dev):
+            rc = _lib.load().b200tp_embedding_fwd(C.byref(a), rows.data_ptr(), out.data_ptr(), _lib.stream(dev),
+                                                  device_status(dev).data_ptr())
+        _lib.check(rc)
+        ctx.save_for_backward(ids)
+        ctx.rule = v, d, weight.dtype, scale, padding
+        ctx.set_materialize_grads(False)
+        return out
+
+    @staticmethod
+    def backward(ctx, d_out):
+        if d_out is None:
+            return None, None, None, None
+        if torch.is_grad_enabled():
+            raise EmbeddingInputError("embedding_lookup has no second derivative (create_graph=True)")
+        VJP_CALLS["embedding_lookup"] = VJP_CALLS.get("embedding_lookup", 0) + 1
+        ids, = ctx.saved_tensors
+        v, d, dtype, scale, padding = ctx.rule
+        dev = ids.device
+        lib = _lib.load()
+        rows = _rows(d_out)
+        grad = torch.empty((v, d), dtype=dtype, device=dev)
+        a = _lib.EmbeddingArgs(ids.data_ptr(), ids.shape[0], v, d, dtype == torch.bfloat16, ids.dtype == torch.int64, scale, rows.stride(0),
+                               padding)
+        nbytes = lib.b200tp_embedding_bwd_workspace_bytes(C.byref(a))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        with _lib.on(dev):
+            rc = lib.b200tp_embedding_bwd(C.byref(a), rows.data_ptr(), grad.data_ptr(), ws.data_ptr(), nbytes, _lib.stream(dev),
+                                          device_status(dev).data_ptr())
+        _lib.check(rc)
+        return grad, None, None, None
+
+
+def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, padding_idx: int | None = None,
+                     validate_ids: bool = False) -> torch.Tensor:
+    """`scale * weight[ids]`, shaped `ids.shape + (D,)`, fp32 arithmetic rounded once to the table's dtype (fp32 or bf16).
+
+    ids: integers of any shape on the table's device (int32 and int64 are read as they are).  `padding_idx`: that row gets no gradient.  An id
+    outside [0, V) gives a row of zeros and no gradient, and `core.loss.check_device_status()` reports it; `validate_ids=True`
+    raises before the launch, with a host synchronisation.  The gradient is dense (V, D)."""
+    if weight.ndim != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise EmbeddingInputError(f"weight must be (V, D), got {tuple(weight.shape)}")
+    if not weight.is_cuda:
+        raise EmbeddingInputError(f"weight must be a CUDA tensor (the operator has no CPU path); got {weight.device}")
+    if weight.dtype not in _DTYPES:
+        raise EmbeddingInputError(f"weight must be fp32 or bf16, got {weight.dtype}")
+    if ids.device != weight.device:
+        raise EmbeddingInputError(f"ids are on {ids.device}, weight on {weight.device}")
+    if ids.dtype not in (torch.int64, torch.int32):
+        if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
+            raise EmbeddingInputError(f"ids must be an integer dtype, got {ids.dtype}")
+        ids = ids.to(torch.int64)
+    v, d = weight.shape
+    padding = -1
+    if padding_idx is not None:
+        if not -v <= padding_idx < v:
+            raise EmbeddingInputError(f"padding_idx must lie in [-{v}, {v}), got {padding_idx}")
+        padding = int(padding_idx) % v
+    if validate_ids and ids.numel() > 0:
+        lo, hi = int(ids.min()), int(ids.max())
+        if lo < 0 or hi >= v:
+            raise EmbeddingInputError(f"ids must satisfy 0 <= id < V={v}; got range [{lo}, {hi}]")
+    return _Lookup.apply(weight, ids.reshape(-1), float(scale), padding).view(*ids.shape, d)

@@ -70,6 +70,8 @@ const char* b200tp_status_string(int code) {
     case B200TP_ERR_CUDA: return "CUDA error";
     case B200TP_ERR_NO_DEVICE: return "no sm_100 device";
     case B200TP_ERR_OPTIM_INPUT: return "optimizer input error";
+    case B200TP_ERR_EMBEDDING_INPUT: return "embedding input error";
+    case B200TP_DEV_BAD_INDEX: return "an embedding id lies outside the table";
     case B200TP_DEV_TIMEOUT_PRODUCER: return "device wait timed out (TMA producer)";
     case B200TP_DEV_TIMEOUT_MMA: return "device wait timed out (MMA issuer)";
     case B200TP_DEV_TIMEOUT_EPILOGUE: return "device wait timed out (epilogue)";

@@ -1,0 +1,488 @@
+// Embedding lookup with scaling, and the gradient of its table by sorted tokens: what the adapters' trunk begins with
+// (adapters/mlx_lm.py:140-164 of the reference calls the model's own embedding module).
+//
+// Forward: y_i = scale W[id_i], a read and a write of N rows.  Backward: dW[v] = scale sum of dy_i over the i with id_i = v, in the order
+// of i, held in fp32 and rounded once; it reads N rows and writes all V rows, nearly all of them zero, so the writes bound
+// it.  No atomics, so equal calls give equal bits:
+//   1. one cluster sorts the tokens by id (stable, least digits first) while all other CTAs fill the table with zeros: the sort's
+//      dependent steps hide behind the fill (V = 151936, D = 4096: 190 us of writes, some 15 us of sort);
+//   2. windows of the sorted tokens sum the rows of each run of equal ids; a run that lies in one window is written, one that
+//      crosses a border leaves a partial sum;
+//   3. the partial sums of runs that cross borders are joined in order.  A padding id that fills half a batch is thousands
+//      of rows: step 2 spreads them over all SMs, and one CTA for 512 columns adds up what is left of them.
+//
+// An id outside [0, V) gives a row of zeros, no gradient, and a status word.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "common.h"
+#include "ptx.cuh"
+
+namespace b200tp {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kCluster = 8;
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kMaxDigit = 9;                       // bits of a sort's digit: 32 warps x 512 counters are 64 kB
+constexpr long long kFillBytes = 256 << 10;        // of one CTA
+constexpr int kCols = 8;                           // columns of a thread
+constexpr int kThreads = 256;
+constexpr int kSlice = kThreads * kCols;           // columns of a CTA that sums
+constexpr int kJoinThreads = 128;
+constexpr int kJoinSlice = kJoinThreads * 4;
+
+__device__ __forceinline__ float value(float x) { return x; }
+__device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// Eight columns of a row.  VEC: adjacent ones from `col`, 16-byte loads; else `col + j * step`, those below d.
+template <typename T, bool VEC>
+struct Cols {
+  uint4 raw[VEC ? sizeof(T) / 2 : 1];
+  T one[VEC ? 1 : kCols];
+
+  __device__ __forceinline__ void load(const T* row, int col, int step, int d) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+        raw[i] = col < d ? __ldg(reinterpret_cast<const uint4*>(row + col) + i) : make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) one[j] = col + j * step < d ? row[col + j * step] : T(0.f);
+    }
+  }
+  __device__ __forceinline__ void add_to(float (&acc)[kCols]) const {
+    float v[kCols];
+    get(v);
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) acc[j] += v[j];
+  }
+  __device__ __forceinline__ void get(float (&v)[kCols]) const {
+    if constexpr (!VEC) {
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) v[j] = value(one[j]);
+    } else if constexpr (sizeof(T) == 2) {
+      const uint32_t w[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+    } else {
+      const uint4 a = raw[0], b = raw[1];
+      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+    }
+  }
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_cols(T* row, int col, int step, int d, const float (&v)[kCols], float scale) {
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int j = 0; j < kCols; ++j)
+      if (col + j * step < d) put(row + col + j * step, v[j] * scale);
+  } else if (col < d) {
+    if constexpr (sizeof(T) == 2) {
+      uint4 u;
+      __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(v[2 * j] * scale, v[2 * j + 1] * scale);
+      *reinterpret_cast<uint4*>(row + col) = u;
+    } else {
+      *reinterpret_cast<float4*>(row + col) = make_float4(v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale);
+      *(reinterpret_cast<float4*>(row + col) + 1) = make_float4(v[4] * scale, v[5] * scale, v[6] * scale, v[7] * scale);
+    }
+  }
+}
+
+// A warp takes 4 x 256 columns of one row (VEC: four loads of 16 bytes or more in flight for each lane).
+template <typename T, typename ID, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+embed_fwd_kernel(const ID* __restrict__ ids, const T* __restrict__ weight, long long w_stride, long long n, int d, int parts,
+                 long long v, float scale, T* __restrict__ out, int* status) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const long long item = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const long long row = item / parts;
+  if (row >= n) return;
+  const int first = static_cast<int>(item - row * parts) * 1024;
+  const long long id = static_cast<long long>(ids[row]);
+  const bool ok = id >= 0 && id < v;
+  if (!ok && lane == 0 && status != nullptr) *status = B200TP_DEV_BAD_INDEX;
+  const T* from = weight + (ok ? id : 0) * w_stride;
+  T* to = out + row * d;
+  Cols<T, VEC> c[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) c[k].load(from, VEC ? first + (k * 32 + lane) * kCols : first + k * 256 + lane, 32, ok ? d : 0);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float x[kCols];
+    c[k].get(x);
+    store_cols<T, VEC>(to, VEC ? first + (k * 32 + lane) * kCols : first + k * 256 + lane, 32, d, x, scale);
+  }
+}
+
+struct Sort {
+  unsigned *key_a, *pos_a, *key_b, *pos_b;   // of n entries each: passes write a, b, a, ...
+  long long n;
+  long long v;                               // keys: ids in [0, v), and v for tokens without a gradient
+  long long padding;                         // an id without a gradient, or -1
+  int digit, passes;
+};
+
+template <typename ID>
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads)
+embed_sort_fill_kernel(const ID* __restrict__ ids, const Sort s, uint4* __restrict__ fill, long long fill_bytes, int* status) {
+  griddep_wait();
+  griddep_launch_dependents();
+  if (blockIdx.x >= kCluster) {              // zeros; whole clusters do this
+    const long long from = (blockIdx.x - kCluster) * kFillBytes / 16, to = min(from + kFillBytes / 16, fill_bytes / 16);
+    for (long long i = from + threadIdx.x; i < to; i += kSortThreads) fill[i] = make_uint4(0, 0, 0, 0);
+    const long long rest = fill_bytes & 15;  // elements are of 2 or 4 bytes
+    if (blockIdx.x == kCluster && threadIdx.x < rest / 2)
+      reinterpret_cast<unsigned short*>(fill)[fill_bytes / 16 * 8 + threadIdx.x] = 0;
+    return;
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  extern __shared__ unsigned shared[];
+  const int bins = 1 << s.digit;
+  unsigned* counts = shared;                 // [warp][bin]: tokens of this digit before the warp's next one, in this CTA
+  unsigned* totals = counts + kSortWarps * bins;   // [bin]: of this CTA
+  unsigned* bases = totals + bins;           // [bin]: place of this CTA's first token of this digit
+  __shared__ unsigned sums[kSortWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster.block_rank());
+  // a warp's tokens are adjacent, so that an order by (digit, warp, place) is stable
+  const long long per = ((s.n + kCluster * kSortWarps - 1) / (kCluster * kSortWarps) + 31) / 32 * 32;
+  const long long lo = min((rank * kSortWarps + warp) * per, s.n), hi = min(lo + per, s.n);
+  unsigned* mine = counts + warp * bins;
+  const unsigned none = 0xffffffffu;
+
+  for (int pass = 0; pass < s.passes; ++pass) {
+    const unsigned* key_in = pass & 1 ? s.key_a : s.key_b;
+    const unsigned* pos_in = pass & 1 ? s.pos_a : s.pos_b;
+    unsigned* key_out = pass & 1 ? s.key_b : s.key_a;
+    unsigned* pos_out = pass & 1 ? s.pos_b : s.pos_a;
+    const int shift = pass * s.digit;
+    auto key_at = [&](long long i) -> unsigned {
+      if (pass > 0) return __ldcg(key_in + i);                    // written by other CTAs of the cluster
+      const long long id = static_cast<long long>(ids[i]);
+      if (id >= 0 && id < s.v) return static_cast<unsigned>(id == s.padding ? s.v : id);
+      if (status != nullptr) *status = B200TP_DEV_BAD_INDEX;
+      return static_cast<unsigned>(s.v);
+    };
+    for (int b = threadIdx.x; b < kSortWarps * bins; b += kSortThreads) counts[b] = 0;
+    __syncthreads();
+    for (long long i = lo + lane; i < hi + lane; i += 32) {       // whole warps; lanes past the end have a digit of their own
+      const bool in = i < hi;
+      const unsigned digit = in ? (key_at(i) >> shift) & (bins - 1) : none;
+      const unsigned peers = __match_any_sync(0xffffffffu, digit);
+      if (in && lane == __ffs(peers) - 1) mine[digit] += __popc(peers);
+      __syncwarp();
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += kSortThreads) {      // counts -> tokens of this digit in warps before; totals
+      unsigned run = 0;
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) {
+        const unsigned c = counts[w * bins + b];
+        counts[w * bins + b] = run;
+        run += c;
+      }
+      totals[b] = run;
+    }
+    cluster.sync();
+    unsigned before = 0, all = 0;                                  // bins <= kSortThreads: one bin a thread
+    if (threadIdx.x < bins) {
+#pragma unroll
+      for (int r = 0; r < kCluster; ++r) {
+        const unsigned c = cluster.map_shared_rank(totals, r)[threadIdx.x];
+        all += c;
+        if (r < rank) before += c;
+      }
+    }
+    unsigned scan = all;                                           // sum over bins up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned up = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += up;
+    }
+    if (lane == 31) sums[warp] = scan;
+    __syncthreads();
+    unsigned below = 0;
+    for (int w = 0; w < warp; ++w) below += sums[w];
+    if (threadIdx.x < bins) bases[threadIdx.x] = below + scan - all + before;
+    __syncthreads();
+    for (long long i = lo + lane; i < hi + lane; i += 32) {
+      const bool in = i < hi;
+      const unsigned key = in ? key_at(i) : none, digit = in ? (key >> shift) & (bins - 1) : none;
+      const unsigned pos = in && pass > 0 ? __ldcg(pos_in + i) : static_cast<unsigned>(i);
+      const unsigned peers = __match_any_sync(0xffffffffu, digit);
+      const unsigned at = in ? bases[digit] + mine[digit] + __popc(peers & ((1u << lane) - 1)) : 0;
+      __syncwarp();
+      if (in && lane == __ffs(peers) - 1) mine[digit] += __popc(peers);
+      __syncwarp();
+      if (in) {
+        key_out[at] = key;
+        pos_out[at] = pos;
+      }
+    }
+    __threadfence();
+    cluster.sync();                                                // the next pass reads what all eight wrote, and counts anew
+  }
+}
+
+// One window of sorted tokens and 2048 columns to a CTA.  Runs that end or begin outside the window leave their sum in `head` (they
+// began before it) or `tail` (they begin in it and go on).
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+embed_sum_kernel(const unsigned* __restrict__ keys, const unsigned* __restrict__ pos, long long n, int window, long long v,
+                 const T* __restrict__ dy, long long dy_stride, int d, float scale, T* __restrict__ dw, float* __restrict__ head,
+                 float* __restrict__ tail) {
+  griddep_wait();
+  griddep_launch_dependents();
+  constexpr int kMost = 64;
+  __shared__ unsigned key_s[kMost + 2], pos_s[kMost];
+  const long long first = static_cast<long long>(blockIdx.x) * window;
+  const int count = static_cast<int>(min(static_cast<long long>(window), n - first));
+  const unsigned none = 0xffffffffu;                               // no key: ids stop below 2^31
+  for (int i = threadIdx.x; i < count + 2; i += kThreads) {
+    const long long at = first + i - 1;
+    key_s[i] = at >= 0 && at < n ? keys[at] : none;
+    if (i >= 1 && i <= count) pos_s[i - 1] = pos[at];
+  }
+  __syncthreads();
+  const int col = blockIdx.y * kSlice + (VEC ? threadIdx.x * kCols : threadIdx.x);
+  if (col >= d) return;
+  constexpr int kAhead = 4;
+  float acc[kCols] = {};
+  bool from_before = key_s[1] == key_s[0];
+  for (int base = 0; base < count; base += kAhead) {
+    Cols<T, VEC> c[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const bool use = base + k < count && key_s[base + k + 1] < v;
+      c[k].load(dy + static_cast<long long>(use ? pos_s[base + k] : 0) * dy_stride, col, kThreads, use ? d : 0);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = base + k;
+      if (i >= count) break;
+      const unsigned key = key_s[i + 1];
+      if (key >= v) return;                                        // tokens without a gradient are the last ones
+      c[k].add_to(acc);
+      const bool goes_on = key_s[i + 2] == key;
+      if (goes_on && i + 1 < count) continue;
+      if (goes_on || from_before) {
+        float* to = (from_before ? head : tail) + static_cast<long long>(blockIdx.x) * d;
+        store_cols<float, VEC>(to, col, kThreads, d, acc, 1.f);
+      } else {
+        store_cols<T, VEC>(dw + key * static_cast<long long>(d), col, kThreads, d, acc, scale);
+      }
+      from_before = false;
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
+    }
+  }
+}
+
+// Runs that begin in a window and go on: tail of that window, heads of the windows up to the run's end.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kJoinThreads)
+embed_join_kernel(const unsigned* __restrict__ keys, long long n, int window, long long v, int d, float scale,
+                  const float* __restrict__ head, const float* __restrict__ tail, T* __restrict__ dw) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const long long w = blockIdx.x, first = w * window, next = first + window;
+  if (next >= n) return;
+  const unsigned key = keys[next - 1];
+  if (key >= v || keys[next] != key) return;                       // no run goes on
+  if (keys[first] == key && w > 0 && keys[first - 1] == key) return;   // it began before
+  long long lo = next + 1, hi = n;                                 // the run's end: the first key above
+  while (lo < hi) {
+    const long long mid = (lo + hi) >> 1;
+    if (keys[mid] == key) lo = mid + 1;
+    else hi = mid;
+  }
+  const long long last = (lo - 1) / window;
+  for (int j = 0; j < (VEC ? 1 : 4); ++j) {
+    const int col = blockIdx.y * kJoinSlice + (VEC ? threadIdx.x * 4 : threadIdx.x + j * kJoinThreads);
+    if (col >= d) return;
+    if constexpr (VEC) {
+      float4 acc = *reinterpret_cast<const float4*>(tail + w * d + col);
+#pragma unroll 8
+      for (long long u = w + 1; u <= last; ++u) {
+        const float4 h = *reinterpret_cast<const float4*>(head + u * d + col);
+        acc.x += h.x; acc.y += h.y; acc.z += h.z; acc.w += h.w;
+      }
+      T* to = dw + key * static_cast<long long>(d) + col;
+      put(to, acc.x * scale);
+      put(to + 1, acc.y * scale);
+      put(to + 2, acc.z * scale);
+      put(to + 3, acc.w * scale);
+    } else {
+      float acc = tail[w * d + col];
+#pragma unroll 8
+      for (long long u = w + 1; u <= last; ++u) acc += head[u * d + col];
+      put(dw + key * static_cast<long long>(d) + col, acc * scale);
+    }
+  }
+}
+
+struct Plan {
+  int window, slices, digit, passes;
+  long long windows;
+  size_t list, partials;                     // bytes of one list of n entries, of head or of tail
+};
+
+// Windows: short enough that about four CTAs an SM have one, between 8 and 64 tokens (a longer one leaves fewer partial sums).
+Plan plan_of(long long n, int d, long long v) {
+  Plan p;
+  p.slices = static_cast<int>(ceil_div(d, kSlice));
+  const long long fit = n * p.slices / (4ll * sm_count());
+  p.window = 8;
+  while (p.window < 64 && p.window * 2 <= fit) p.window *= 2;
+  p.windows = ceil_div(n, p.window);
+  int bits = 1;
+  while ((v >> bits) != 0) ++bits;           // keys are 0 to v
+  p.passes = static_cast<int>(ceil_div(bits, kMaxDigit));
+  p.digit = static_cast<int>(ceil_div(bits, p.passes));
+  p.list = align_up(static_cast<size_t>(n) * 4, 256);
+  p.partials = align_up(static_cast<size_t>(p.windows) * d * 4, 256);
+  return p;
+}
+
+int check(const b200tp_embedding_args* a) {
+  if (a == nullptr) return fail(B200TP_ERR_EMBEDDING_INPUT, "args is null");
+  if (a->dtype != B200TP_F32 && a->dtype != B200TP_BF16) return fail(B200TP_ERR_EMBEDDING_INPUT, "tables must be fp32 or bf16");
+  if (a->n < 0 || a->n > (1ll << 30)) return fail(B200TP_ERR_EMBEDDING_INPUT, "the number of tokens must lie in [0, 2^30]");
+  if (a->d < 1 || a->d > (1 << 20)) return fail(B200TP_ERR_EMBEDDING_INPUT, "rows must have 1 to 2^20 columns");
+  if (a->v < 1 || a->v >= (1ll << 31) - 1) return fail(B200TP_ERR_EMBEDDING_INPUT, "the table must have 1 to 2^31 - 2 rows");
+  if (a->ids == nullptr && a->n > 0) return fail(B200TP_ERR_EMBEDDING_INPUT, "ids is null");
+  if (a->row_stride < 0) return fail(B200TP_ERR_EMBEDDING_INPUT, "negative row stride");
+  return B200TP_OK;
+}
+
+bool wide(const void* a, const void* b, long long stride, int d, int item) {
+  return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0 && stride * item % 16 == 0 && d % kCols == 0;
+}
+
+template <typename T, typename ID>
+int launch_fwd(const b200tp_embedding_args* a, const void* weight, void* out, cudaStream_t stream, int* status) {
+  const int parts = static_cast<int>(ceil_div(a->d, 1024));
+  const long long blocks = ceil_div(a->n * parts, kThreads / 32);
+  if (blocks > (1ll << 31) - 1) return fail(B200TP_ERR_EMBEDDING_INPUT, "too many tokens for one launch");
+  auto go = [&](auto kernel) {
+    return launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, static_cast<const ID*>(a->ids),
+                      static_cast<const T*>(weight), a->row_stride, a->n, a->d, parts, a->v, a->scale, static_cast<T*>(out), status);
+  };
+  B200TP_CUDA_OK(wide(weight, out, a->row_stride, a->d, sizeof(T)) ? go(embed_fwd_kernel<T, ID, true>) : go(embed_fwd_kernel<T, ID, false>));
+  return B200TP_OK;
+}
+
+template <typename ID>
+int launch_sort(const b200tp_embedding_args* a, const Sort& s, void* dw, cudaStream_t stream, int* status) {
+  const long long bytes = a->v * a->d * (a->dtype == B200TP_BF16 ? 2 : 4);
+  const size_t smem = static_cast<size_t>(kSortWarps + 2) * (size_t{4} << s.digit);
+  B200TP_CUDA_OK(cudaFuncSetAttribute(embed_sort_fill_kernel<ID>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  const long long blocks = kCluster + ceil_div(ceil_div(bytes, kFillBytes), kCluster) * kCluster;
+  B200TP_CUDA_OK(launch_pdl(embed_sort_fill_kernel<ID>, dim3(static_cast<unsigned>(blocks)), dim3(kSortThreads), smem, stream,
+                            static_cast<const ID*>(a->ids), s, static_cast<uint4*>(dw), bytes, status));
+  return B200TP_OK;
+}
+
+template <typename T>
+int launch_sums(const b200tp_embedding_args* a, const Plan& p, const unsigned* keys, const unsigned* pos, const void* dy, void* dw,
+                float* head, float* tail, cudaStream_t stream) {
+  const bool vec = wide(dy, dw, a->row_stride, a->d, sizeof(T));
+  const dim3 grid(static_cast<unsigned>(p.windows), p.slices);
+  auto sum = [&](auto kernel) {
+    return launch_pdl(kernel, grid, dim3(kThreads), 0, stream, keys, pos, a->n, p.window, a->v, static_cast<const T*>(dy), a->row_stride,
+                      a->d, a->scale, static_cast<T*>(dw), head, tail);
+  };
+  B200TP_CUDA_OK(vec ? sum(embed_sum_kernel<T, true>) : sum(embed_sum_kernel<T, false>));
+  if (p.windows == 1) return B200TP_OK;
+  const dim3 join_grid(static_cast<unsigned>(p.windows), static_cast<unsigned>(ceil_div(a->d, kJoinSlice)));
+  auto join = [&](auto kernel) {
+    return launch_pdl(kernel, join_grid, dim3(kJoinThreads), 0, stream, keys, a->n, p.window, a->v, a->d, a->scale, head, tail,
+                      static_cast<T*>(dw));
+  };
+  B200TP_CUDA_OK(vec ? join(embed_join_kernel<T, true>) : join(embed_join_kernel<T, false>));
+  return B200TP_OK;
+}
+
+}  // namespace
+}  // namespace b200tp
+
+using namespace b200tp;
+
+extern "C" {
+
+int b200tp_embedding_fwd(const b200tp_embedding_args* a, const void* weight, void* out, void* stream_v, int* status) {
+  int rc = check(a);
+  if (rc) return rc;
+  if (a->n == 0) return B200TP_OK;
+  if (weight == nullptr || out == nullptr) return fail(B200TP_ERR_EMBEDDING_INPUT, "weight / out is null");
+  rc = require_sm100();
+  if (rc) return rc;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  if (a->dtype == B200TP_BF16)
+    return a->ids_int64 ? launch_fwd<__nv_bfloat16, long long>(a, weight, out, stream, status)
+                        : launch_fwd<__nv_bfloat16, int>(a, weight, out, stream, status);
+  return a->ids_int64 ? launch_fwd<float, long long>(a, weight, out, stream, status)
+                      : launch_fwd<float, int>(a, weight, out, stream, status);
+}
+
+size_t b200tp_embedding_bwd_workspace_bytes(const b200tp_embedding_args* a) {
+  if (check(a) != B200TP_OK || a->n == 0) return 0;
+  const Plan p = plan_of(a->n, a->d, a->v);
+  return 4 * p.list + 2 * p.partials;
+}
+
+int b200tp_embedding_bwd(const b200tp_embedding_args* a, const void* d_out, void* d_weight, void* workspace,
+                         size_t workspace_bytes, void* stream_v, int* status) {
+  int rc = check(a);
+  if (rc) return rc;
+  if (d_weight == nullptr || (d_out == nullptr && a->n > 0)) return fail(B200TP_ERR_EMBEDDING_INPUT, "d_out / d_weight is null");
+  if ((reinterpret_cast<uintptr_t>(d_weight) & 15) != 0) return fail(B200TP_ERR_EMBEDDING_INPUT, "d_weight must be 16-byte aligned");
+  const size_t need = b200tp_embedding_bwd_workspace_bytes(a);
+  if (need > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 || workspace_bytes < need))
+    return fail(B200TP_ERR_WORKSPACE, "embedding backward workspace missing, misaligned or smaller than " + std::to_string(need) + " bytes");
+  rc = require_sm100();
+  if (rc) return rc;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  if (a->n == 0) {
+    B200TP_CUDA_OK(cudaMemsetAsync(d_weight, 0, static_cast<size_t>(a->v) * a->d * (a->dtype == B200TP_BF16 ? 2 : 4), stream));
+    return B200TP_OK;
+  }
+  const Plan p = plan_of(a->n, a->d, a->v);
+  char* ws = static_cast<char*>(workspace);
+  Sort s;
+  s.key_a = reinterpret_cast<unsigned*>(ws);
+  s.pos_a = reinterpret_cast<unsigned*>(ws + p.list);
+  s.key_b = reinterpret_cast<unsigned*>(ws + 2 * p.list);
+  s.pos_b = reinterpret_cast<unsigned*>(ws + 3 * p.list);
+  float* head = reinterpret_cast<float*>(ws + 4 * p.list);
+  float* tail = reinterpret_cast<float*>(ws + 4 * p.list + p.partials);
+  s.n = a->n;
+  s.v = a->v;
+  s.padding = a->padding_idx;
+  s.digit = p.digit;
+  s.passes = p.passes;
+  rc = a->ids_int64 ? launch_sort<long long>(a, s, d_weight, stream, status) : launch_sort<int>(a, s, d_weight, stream, status);
+  if (rc) return rc;
+  const unsigned* keys = p.passes & 1 ? s.key_a : s.key_b;
+  const unsigned* pos = p.passes & 1 ? s.pos_a : s.pos_b;
+  return a->dtype == B200TP_BF16 ? launch_sums<__nv_bfloat16>(a, p, keys, pos, d_out, d_weight, head, tail, stream)
+                                 : launch_sums<float>(a, p, keys, pos, d_out, d_weight, head, tail, stream);
+}
+
+}  // extern "C"

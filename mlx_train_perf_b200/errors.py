@@ -33,6 +33,10 @@ class OptimizerInputError(MlxTrainPerfError):
     """Shape/dtype/layout validation failure at the optimizer boundary."""
 
 
+class EmbeddingInputError(MlxTrainPerfError):
+    """Shape/dtype/id-range validation failure at the embedding boundary."""
+
+
 class PackingError(MlxTrainPerfError):
     """Sequence-packing input validation failure."""
 

@@ -1,4 +1,4 @@
-"""Refusals of the objectives' and the optimizer's C entry points, which come before anything is launched (no GPU needed), and the
+"""Refusals of the objectives', the optimizer's and the embedding's C entry points, which come before anything is launched (no GPU needed), and the
 Python checks that host tensors reach."""
 import ctypes as C
 
@@ -6,7 +6,8 @@ import numpy as np
 import pytest
 import torch
 
-from mlx_train_perf_b200 import AdamW, AdamWState, LossInputError, OptimizerInputError, _lib, policy_loss, preference_loss
+from mlx_train_perf_b200 import (AdamW, AdamWState, EmbeddingInputError, LossInputError, OptimizerInputError, _lib, embedding_lookup,
+                                 policy_loss, preference_loss)
 from mlx_train_perf_b200.build import build
 
 PTR = 1 << 20                          # a non-null placeholder: nothing is dereferenced
@@ -92,8 +93,39 @@ def test_adamw_of_nothing(lib):
     assert _adamw([]) == _lib.OK
 
 
+def _embedding(**change):
+    a = _lib.EmbeddingArgs(PTR, 100, 1000, 64, 1, 1, 1.0, 64, -1)
+    for k, v in change.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("change", [dict(ids=None), dict(n=-1), dict(n=(1 << 30) + 1), dict(v=0), dict(v=1 << 31), dict(d=0), dict(d=1 << 21),
+                                    dict(dtype=2), dict(row_stride=-1)])
+def test_embedding_arguments(lib, change):
+    a = C.byref(_embedding(**change))
+    assert lib.b200tp_embedding_bwd_workspace_bytes(a) == 0
+    assert lib.b200tp_embedding_fwd(a, PTR, PTR, None, None) == _lib.ERR_EMBEDDING_INPUT
+    assert lib.b200tp_embedding_bwd(a, PTR, PTR, PTR, 1 << 30, None, None) == _lib.ERR_EMBEDDING_INPUT
+
+
+def test_embedding_pointers_and_workspace(lib):
+    a = _embedding()
+    need = lib.b200tp_embedding_bwd_workspace_bytes(C.byref(a))
+    # keys and places twice, and two partial sums of a row for each window of 8 tokens at least
+    assert 16 * 100 <= need <= 4 * 512 + 2 * (13 * 64 * 4 + 256)
+    bwd = lambda dy=PTR, dw=PTR, ws=PTR, n=need: lib.b200tp_embedding_bwd(C.byref(a), dy, dw, ws, n, None, None)
+    assert bwd(dy=None) == bwd(dw=None) == bwd(dw=PTR + 8) == _lib.ERR_EMBEDDING_INPUT
+    assert bwd(ws=None) == bwd(ws=PTR + 16) == bwd(n=need - 1) == _lib.ERR_WORKSPACE
+    assert lib.b200tp_embedding_fwd(C.byref(a), None, PTR, None, None) == _lib.ERR_EMBEDDING_INPUT
+    assert lib.b200tp_embedding_fwd(C.byref(_embedding(n=0, ids=None)), None, None, None, None) == _lib.OK
+
+
 def test_status_text(lib):
     assert lib.b200tp_status_string(_lib.ERR_OPTIM_INPUT) == b"optimizer input error"
+    assert lib.b200tp_status_string(_lib.ERR_EMBEDDING_INPUT) == b"embedding input error"
+    with pytest.raises(EmbeddingInputError, match="outside the table"):
+        _lib.raise_for_device_status(_lib.DEV_BAD_INDEX)
 
 
 def test_host_tensors_are_refused():
@@ -102,6 +134,8 @@ def test_host_tensors_are_refused():
         preference_loss(x)
     with pytest.raises(LossInputError, match="CUDA"):
         policy_loss(x, x, a)
+    with pytest.raises(EmbeddingInputError, match="CUDA"):
+        embedding_lookup(torch.zeros(3, dtype=torch.int64), x)
     with pytest.raises(OptimizerInputError, match="CUDA"):
         AdamWState.zeros([x])
     p = torch.nn.Parameter(x)
