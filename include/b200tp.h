@@ -374,10 +374,10 @@ int b200tp_preference_loss_fwd(const b200tp_objective_args* a, int32_t kind, dou
 /* Clipped policy loss: per taken token -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef kl, r = exp(logps -
  * old_logps), kl of logps against ref_logps (K1: logps - ref, K2: half its square, K3: exp(-d) + d - 1 for
  * that difference d); averaged over all taken tokens, over each sequence's and then the sequences, or summed.
- * out3: loss, mean kl and share of clipped tokens, both over the taken tokens.  slopes (NULL: no gradient wanted): f32 a
+ * loss: one f32; stats: mean kl and share of clipped tokens, both over the taken tokens.  slopes (NULL: no gradient wanted): f32 a
  * token, (seqs, length) or (length,); weights: f32, (seqs,) for NORMALIZE_SEQUENCE (then per_sequence 1), else (1,). */
 int b200tp_policy_loss_fwd(const b200tp_objective_args* a, double clip_low, double clip_high, double kl_coef, int32_t kl_kind,
-                           int32_t normalize, float* out3, float* slopes, float* weights, void* workspace,
+                           int32_t normalize, float* loss, float* stats, float* slopes, float* weights, void* workspace,
                            size_t workspace_bytes, void* stream);
 
 /* Gradient of either loss for logps (contiguous, `dtype`, every token written): upstream[0] * weight * slope, a taken

@@ -159,8 +159,8 @@ SIGNATURES = {
                                              C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
                                              C.c_void_p]),
     "b200tp_policy_loss_fwd": (C.c_int, [C.POINTER(ObjectiveArgs), C.c_double, C.c_double, C.c_double, C.c_int32,
-                                         C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
-                                         C.c_void_p]),
+                                         C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                         C.c_size_t, C.c_void_p]),
     "b200tp_objective_bwd": (C.c_int, [C.POINTER(ObjectiveArgs), C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p,
                                        C.c_void_p, C.c_void_p]),
 }

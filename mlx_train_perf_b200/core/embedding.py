@@ -23,29 +23,28 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 class _Lookup(torch.autograd.Function):
-    """(weight, ids (N,), scale, padding) -> (N, D)."""
+    """(weight, ids, scale, padding) -> ids.shape + (D,)."""
 
     @staticmethod
     def forward(ctx, weight, ids, scale, padding):
-        n, (v, d) = ids.shape[0], weight.shape
-        dev = weight.device
+        v, d = weight.shape
+        dev, dtype = weight.device, weight.dtype
         rows = _rows(weight)
-        out = torch.empty((n, d), dtype=weight.dtype, device=dev)
-        a = _lib.EmbeddingArgs(ids.data_ptr(), n, v, d, weight.dtype == torch.bfloat16, ids.dtype == torch.int64, scale, rows.stride(0),
+        out = torch.empty((*ids.shape, d), dtype=dtype, device=dev)
+        if not ids.is_contiguous():
+            ids = ids.contiguous()
+        a = _lib.EmbeddingArgs(ids.data_ptr(), ids.numel(), v, d, dtype is torch.bfloat16, ids.dtype is torch.int64, scale, rows.stride(0),
                                padding)
         with _lib.on(dev):
             rc = _lib.load().b200tp_embedding_fwd(C.byref(a), rows.data_ptr(), out.data_ptr(), _lib.stream(dev),
                                                   device_status(dev).data_ptr())
         _lib.check(rc)
         ctx.save_for_backward(ids)
-        ctx.rule = v, d, weight.dtype, scale, padding
-        ctx.set_materialize_grads(False)
+        ctx.rule = v, d, dtype, scale, padding
         return out
 
     @staticmethod
     def backward(ctx, d_out):
-        if d_out is None:
-            return None, None, None, None
         if torch.is_grad_enabled():
             raise EmbeddingInputError("embedding_lookup has no second derivative (create_graph=True)")
         VJP_CALLS["embedding_lookup"] = VJP_CALLS.get("embedding_lookup", 0) + 1
@@ -53,9 +52,11 @@ class _Lookup(torch.autograd.Function):
         v, d, dtype, scale, padding = ctx.rule
         dev = ids.device
         lib = _lib.load()
+        if d_out.ndim != 2:
+            d_out = d_out.reshape(-1, d)
         rows = _rows(d_out)
         grad = torch.empty((v, d), dtype=dtype, device=dev)
-        a = _lib.EmbeddingArgs(ids.data_ptr(), ids.shape[0], v, d, dtype == torch.bfloat16, ids.dtype == torch.int64, scale, rows.stride(0),
+        a = _lib.EmbeddingArgs(ids.data_ptr(), ids.numel(), v, d, dtype is torch.bfloat16, ids.dtype is torch.int64, scale, rows.stride(0),
                                padding)
         nbytes = lib.b200tp_embedding_bwd_workspace_bytes(C.byref(a))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
@@ -95,4 +96,4 @@ def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 
         lo, hi = int(ids.min()), int(ids.max())
         if lo < 0 or hi >= v:
             raise EmbeddingInputError(f"ids must satisfy 0 <= id < V={v}; got range [{lo}, {hi}]")
-    return _Lookup.apply(weight, ids.reshape(-1), float(scale), padding).view(*ids.shape, d)
+    return _Lookup.apply(weight, ids, float(scale), padding)

@@ -71,24 +71,23 @@ def _check_tokens(logps: torch.Tensor, cu_seqlens: torch.Tensor | None, validate
 def _check_like(name: str, t: torch.Tensor, logps: torch.Tensor) -> torch.Tensor:
     if t.shape != logps.shape or t.device != logps.device:
         raise LossInputError(f"{name} must match logps: {tuple(logps.shape)} on {logps.device}, got {tuple(t.shape)} on {t.device}")
-    return _unit_inner(t.detach())
+    return _unit_inner(t)
 
 
-def _check_others(logps, mask, **others):
-    """mask and the other models' log-probabilities, brought to one dtype where they differ (fp32: exact)."""
-    if mask is not None:
-        if mask.dtype != torch.bool:
-            raise LossInputError(f"mask must be bool, got {mask.dtype}")
-        mask = _check_like("mask", mask, logps)
-    given = {k: t for k, t in others.items() if t is not None}
-    for name, t in given.items():
-        if t.dtype not in _DTYPES:
-            raise LossInputError(f"{name} must be fp32 or bf16, got {t.dtype}")
-        given[name] = _check_like(name, t, logps)
-    dtypes = {t.dtype for t in given.values()}
-    if len(dtypes) > 1:
-        given = {k: t.to(torch.float32) for k, t in given.items()}
-    return mask, given
+def _check_mask(mask: torch.Tensor | None, logps: torch.Tensor) -> torch.Tensor | None:
+    if mask is None:
+        return None
+    if mask.dtype != torch.bool:
+        raise LossInputError(f"mask must be bool, got {mask.dtype}")
+    return _check_like("mask", mask, logps)
+
+
+def _check_other(name: str, t: torch.Tensor | None, logps: torch.Tensor) -> torch.Tensor | None:
+    if t is None:
+        return None
+    if t.dtype not in _DTYPES:
+        raise LossInputError(f"{name} must be fp32 or bf16, got {t.dtype}")
+    return _check_like(name, t, logps)
 
 
 def _row_stride(t: torch.Tensor | None) -> int:
@@ -99,7 +98,7 @@ class _Call:
     """What one call hands the library, and what it got back.  The autograd functions below take it as their one argument beside
     `logps`: every further argument and output costs a training step host time (12 arguments and 3 outputs: 15 us of it)."""
     __slots__ = ("seqs", "mask", "cu", "old", "ref", "adv", "adv_strides", "rule", "from_nll", "per_sequence", "recorded", "out",
-                 "shape", "dtype")
+                 "at", "shape", "dtype", "slopes")
 
     def args(self, logps) -> _lib.ObjectiveArgs:
         mask, cu, old, ref, adv = self.mask, self.cu, self.old, self.ref, self.adv
@@ -111,35 +110,41 @@ class _Call:
             _row_stride(ref), _row_stride(mask), *self.adv_strides, logps.dtype == torch.bfloat16,
             other is not None and other.dtype == torch.bfloat16, cu is not None and cu.dtype == torch.int64, self.from_nll)
 
-    def keep(self, ctx, logps, weights, slopes):
-        """Everything the gradient needs; the inputs themselves are let go."""
-        ctx.save_for_backward(weights, slopes, self.mask, self.cu)
-        ctx.call, self.shape, self.dtype = self, logps.shape, logps.dtype
+    def buffer(self, lib, a, logps, slopes: bool) -> tuple[torch.Tensor, int, int, int]:
+        """One allocation for the workspace, the weights of sequences or of the batch, and the tokens' slopes: (buffer, workspace bytes,
+        address of the weights, address of the slopes or 0)."""
+        nbytes = lib.b200tp_objective_workspace_bytes(C.byref(a))
+        self.at = nbytes // 4
+        count = self.seqs if self.per_sequence else 1
+        buf = torch.empty(self.at + count + (logps.numel() if slopes else 0), dtype=torch.float32, device=logps.device)
+        weights = buf.data_ptr() + nbytes
+        return buf, nbytes, weights, weights + 4 * count if slopes else 0
+
+    def keep(self, ctx, logps, buf, slopes: bool):
+        """Everything the gradient needs, apart from what the caller is given and may write to; the inputs are let go."""
+        ctx.save_for_backward(buf, self.mask, self.cu)
+        ctx.call, self.shape, self.dtype, self.slopes = self, logps.shape, logps.dtype, slopes
         self.mask = self.cu = self.old = self.ref = self.adv = None
 
     def gradient(self, ctx, g):
         """Gradient for logps from the loss's upstream gradient.  Addresses are those of the tensors that autograd hands back."""
         if torch.is_grad_enabled():
             raise LossInputError("this loss has no second derivative (create_graph=True)")
-        weights, slopes, mask, cu = ctx.saved_tensors
-        dev = weights.device
-        grad = torch.empty(self.shape, dtype=self.dtype, device=dev)
+        buf, mask, cu = ctx.saved_tensors
+        dev, dtype = buf.device, self.dtype
+        grad = torch.empty(self.shape, dtype=dtype, device=dev)
         at = grad.data_ptr()                              # logps is not read any more
         a = _lib.ObjectiveArgs(at, None, None, None if mask is None else mask.data_ptr(), None, None if cu is None else cu.data_ptr(),
-                               self.seqs, self.shape[-1], 0, 0, 0, _row_stride(mask), 0, 0, self.dtype == torch.bfloat16, 0,
-                               cu is not None and cu.dtype == torch.int64, 0)
-        if g.dtype != torch.float32:
+                               self.seqs, self.shape[-1], 0, 0, 0, _row_stride(mask), 0, 0, dtype is torch.bfloat16, 0,
+                               cu is not None and cu.dtype is torch.int64, 0)
+        if g.dtype is not torch.float32:
             g = g.to(torch.float32)
+        weights = buf.data_ptr() + 4 * self.at
+        slopes = weights + 4 * (self.seqs if self.per_sequence else 1) if self.slopes else None
         with _lib.on(dev):
-            rc = _lib.load().b200tp_objective_bwd(C.byref(a), None if slopes is None else slopes.data_ptr(), weights.data_ptr(),
-                                                  self.per_sequence, g.data_ptr(), at, _lib.stream(dev))
+            rc = _lib.load().b200tp_objective_bwd(C.byref(a), slopes, weights, self.per_sequence, g.data_ptr(), at, _lib.stream(dev))
         _lib.check(rc)
         return grad
-
-
-def _workspace(lib, a, device):
-    nbytes = lib.b200tp_objective_workspace_bytes(C.byref(a))
-    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
 
 
 class _Preference(torch.autograd.Function):
@@ -148,19 +153,18 @@ class _Preference(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logps, call):
         lib = _lib.load()
-        dev, seqs = logps.device, call.seqs
+        dev = logps.device
         a = call.args(logps)
-        out = torch.empty(1 + 2 * seqs, dtype=torch.float32, device=dev)       # loss, rewards, weights
-        ws, nbytes = _workspace(lib, a, dev)
-        base = out.data_ptr()
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        call.out = torch.empty(call.seqs, dtype=torch.float32, device=dev)
+        buf, nbytes, weights, _ = call.buffer(lib, a, logps, False)
         with _lib.on(dev):
-            rc = lib.b200tp_preference_loss_fwd(C.byref(a), *call.rule, base, base + 4, base + 4 + 4 * seqs, ws.data_ptr(), nbytes,
-                                                _lib.stream(dev))
+            rc = lib.b200tp_preference_loss_fwd(C.byref(a), *call.rule, loss.data_ptr(), call.out.data_ptr(), weights, buf.data_ptr(),
+                                                nbytes, _lib.stream(dev))
         _lib.check(rc)
-        call.out = out[1:1 + seqs]
         if call.recorded:
-            call.keep(ctx, logps, out[1 + seqs:], None)
-        return out[0]
+            call.keep(ctx, logps, buf, False)
+        return loss
 
     @staticmethod
     def backward(ctx, g):
@@ -175,20 +179,19 @@ class _Policy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logps, call):
         lib = _lib.load()
-        dev, recorded = logps.device, call.recorded
+        dev = logps.device
         a = call.args(logps)
-        out = torch.empty(3 + (call.seqs if call.per_sequence else 1), dtype=torch.float32, device=dev)   # loss, kl, share; weights
-        slopes = torch.empty(logps.shape, dtype=torch.float32, device=dev) if recorded else None
-        ws, nbytes = _workspace(lib, a, dev)
-        base = out.data_ptr()
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        stats = torch.empty(2, dtype=torch.float32, device=dev)
+        buf, nbytes, weights, slopes = call.buffer(lib, a, logps, call.recorded)
         with _lib.on(dev):
-            rc = lib.b200tp_policy_loss_fwd(C.byref(a), *call.rule, base, slopes.data_ptr() if recorded else None, base + 12,
-                                            ws.data_ptr(), nbytes, _lib.stream(dev))
+            rc = lib.b200tp_policy_loss_fwd(C.byref(a), *call.rule, loss.data_ptr(), stats.data_ptr(), slopes or None, weights,
+                                            buf.data_ptr(), nbytes, _lib.stream(dev))
         _lib.check(rc)
-        call.out = out[1], out[2]
-        if recorded:
-            call.keep(ctx, logps, out[3:], slopes)
-        return out[0]
+        call.out = stats.unbind()
+        if call.recorded:
+            call.keep(ctx, logps, buf, True)
+        return loss
 
     @staticmethod
     def backward(ctx, g):
@@ -196,10 +199,10 @@ class _Policy(torch.autograd.Function):
         return ctx.call.gradient(ctx, g), None
 
 
-def _call(logps, seqs, mask, cu_seqlens, given, rule, from_nll, per_sequence) -> _Call:
+def _call(logps, seqs, mask, cu_seqlens, old, ref, rule, from_nll, per_sequence) -> _Call:
     call = _Call()
     call.seqs, call.mask, call.cu = seqs, mask, None if cu_seqlens is None else cu_seqlens.contiguous()
-    call.old, call.ref = given.get("old_logps"), given.get("ref_logps")
+    call.old, call.ref = old, ref
     call.adv, call.adv_strides, call.rule, call.from_nll, call.per_sequence = None, (0, 0), rule, bool(from_nll), per_sequence
     call.recorded = torch.is_grad_enabled() and logps.requires_grad
     return call
@@ -227,9 +230,9 @@ def preference_loss(logps: torch.Tensor, ref_logps: torch.Tensor | None = None, 
         raise LossInputError(f"beta must be positive, got {beta}")
     if not 0.0 <= label_smoothing < 1.0 or (label_smoothing and kind != "sigmoid"):
         raise LossInputError(f"label_smoothing must lie in [0, 1) and needs kind='sigmoid'; got {label_smoothing} with {kind!r}")
-    mask, given = _check_others(logps, mask, ref_logps=ref_logps)
+    mask, ref = _check_mask(mask, logps), _check_other("ref_logps", ref_logps, logps)
     rule = (_PREFERENCES[kind], float(beta), float(label_smoothing), float(margin), bool(average))
-    call = _call(logps, seqs, mask, cu_seqlens, given, rule, from_nll, True)
+    call = _call(logps, seqs, mask, cu_seqlens, None, ref, rule, from_nll, True)
     loss = _Preference.apply(_unit_inner(logps), call)
     return PreferenceLoss(loss, call.out[:seqs // 2], call.out[seqs // 2:])
 
@@ -256,18 +259,22 @@ def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor, advantages: torch.
         raise LossInputError(f"clip_low must lie in [0, 1] and clip_high be at least 0; got {clip_low}, {clip_high}")
     if kl_coef != 0.0 and ref_logps is None:
         raise LossInputError("a KL term (kl_coef != 0) needs ref_logps")
-    mask, given = _check_others(logps, mask, old_logps=old_logps, ref_logps=ref_logps)
-    adv = advantages.detach()
+    mask, old, ref = (_check_mask(mask, logps), _check_other("old_logps", old_logps, logps),
+                      _check_other("ref_logps", ref_logps, logps))
+    if ref is not None and ref.dtype is not old.dtype:   # the kernel reads both in one dtype
+        old, ref = old.to(torch.float32), ref.to(torch.float32)
+    adv = advantages
     if adv.dtype not in _DTYPES or adv.device != logps.device or (adv.shape != logps.shape and tuple(adv.shape) != (seqs, 1)):
         raise LossInputError(f"advantages must be fp32 / bf16, on logps' device and like logps {tuple(logps.shape)} or ({seqs}, 1); "
                              f"got {tuple(adv.shape)} {adv.dtype} on {adv.device}")
-    adv = adv.to(torch.float32)
+    if adv.dtype is not torch.float32:
+        adv = adv.to(torch.float32)
     if cu_seqlens is None:
         strides = adv.stride(0), adv.stride(1) if adv.shape[1] == logps.shape[1] else 0
     else:
         strides = (0, adv.stride(0)) if adv.ndim == 1 else (adv.stride(0), 0)
     rule = (float(clip_low), float(clip_high), float(kl_coef), _KLS[kl], _NORMALIZE[normalize])
-    call = _call(logps, seqs, mask, cu_seqlens, given, rule, from_nll, normalize == "sequence")
+    call = _call(logps, seqs, mask, cu_seqlens, old, ref, rule, from_nll, normalize == "sequence")
     call.adv, call.adv_strides = adv, strides
     loss = _Policy.apply(_unit_inner(logps), call)
     return PolicyLoss(loss, *call.out)

@@ -4,12 +4,12 @@
 // Forward: y_i = scale W[id_i], a read and a write of N rows.  Backward: dW[v] = scale sum of dy_i over the i with id_i = v, in the order
 // of i, held in fp32 and rounded once; it reads N rows and writes all V rows, nearly all of them zero, so the writes bound
 // it.  No atomics, so equal calls give equal bits:
-//   1. one cluster sorts the tokens by id (stable, least digits first) while all other CTAs fill the table with zeros: the sort's
-//      dependent steps hide behind the fill (V = 151936, D = 4096: 190 us of writes, some 15 us of sort);
+//   1. one cluster sorts the tokens by id (stable, least digits first); beside it a second kernel fills the table with zeros, so that
+//      the sort's dependent steps cost nothing where the table is large (V = 151936, D = 4096: 170 us of writes at 7.3 TB/s);
 //   2. windows of the sorted tokens sum the rows of each run of equal ids; a run that lies in one window is written, one that
 //      crosses a border leaves a partial sum;
 //   3. the partial sums of runs that cross borders are joined in order.  A padding id that fills half a batch is thousands
-//      of rows: step 2 spreads them over all SMs, and one CTA for 512 columns adds up what is left of them.
+//      of rows: step 2 spreads them over all SMs, and one CTA for 256 columns adds up what is left of them.
 //
 // An id outside [0, V) gives a row of zeros, no gradient, and a status word.
 #include <cooperative_groups.h>
@@ -27,13 +27,13 @@ namespace cg = cooperative_groups;
 constexpr int kCluster = 8;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kKeys = 4;                           // keys of a lane in flight
 constexpr int kMaxDigit = 9;                       // bits of a sort's digit: 32 warps x 512 counters are 64 kB
-constexpr long long kFillBytes = 256 << 10;        // of one CTA
+constexpr long long kFillBytes = 64 << 10;         // of one CTA (256 kB: 172 us, 1 MB: 181 us for 1.24 GB)
 constexpr int kCols = 8;                           // columns of a thread
 constexpr int kThreads = 256;
 constexpr int kSlice = kThreads * kCols;           // columns of a CTA that sums
-constexpr int kJoinThreads = 128;
-constexpr int kJoinSlice = kJoinThreads * 4;
+constexpr int kJoinSlice = 256;                    // columns of a CTA that joins
 
 __device__ __forceinline__ float value(float x) { return x; }
 __device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -138,19 +138,25 @@ struct Sort {
   int digit, passes;
 };
 
+// Zeros over the table, while the sort before it in the stream runs: nothing here waits for that one's results.  Whatever came
+// before the sort is over (the sort lets this kernel start only after its own wait), and what comes after this one finds the sort
+// finished because the last CTA here does not end before it.
+__global__ void __launch_bounds__(kSortThreads) embed_fill_kernel(uint4* __restrict__ fill, long long bytes) {
+  griddep_launch_dependents();
+  const long long from = blockIdx.x * (kFillBytes / 16), to = min(from + kFillBytes / 16, bytes / 16);
+  for (long long i = from + threadIdx.x; i < to; i += kSortThreads) fill[i] = make_uint4(0, 0, 0, 0);
+  if (blockIdx.x == gridDim.x - 1) {
+    if (threadIdx.x < (bytes & 15) / 2)                            // elements are of 2 or 4 bytes
+      reinterpret_cast<unsigned short*>(fill)[bytes / 16 * 8 + threadIdx.x] = 0;
+    griddep_wait();
+  }
+}
+
 template <typename ID>
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads)
-embed_sort_fill_kernel(const ID* __restrict__ ids, const Sort s, uint4* __restrict__ fill, long long fill_bytes, int* status) {
+embed_sort_kernel(const ID* __restrict__ ids, const Sort s, int* status) {
   griddep_wait();
   griddep_launch_dependents();
-  if (blockIdx.x >= kCluster) {              // zeros; whole clusters do this
-    const long long from = (blockIdx.x - kCluster) * kFillBytes / 16, to = min(from + kFillBytes / 16, fill_bytes / 16);
-    for (long long i = from + threadIdx.x; i < to; i += kSortThreads) fill[i] = make_uint4(0, 0, 0, 0);
-    const long long rest = fill_bytes & 15;  // elements are of 2 or 4 bytes
-    if (blockIdx.x == kCluster && threadIdx.x < rest / 2)
-      reinterpret_cast<unsigned short*>(fill)[fill_bytes / 16 * 8 + threadIdx.x] = 0;
-    return;
-  }
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ unsigned shared[];
   const int bins = 1 << s.digit;
@@ -181,12 +187,18 @@ embed_sort_fill_kernel(const ID* __restrict__ ids, const Sort s, uint4* __restri
     };
     for (int b = threadIdx.x; b < kSortWarps * bins; b += kSortThreads) counts[b] = 0;
     __syncthreads();
-    for (long long i = lo + lane; i < hi + lane; i += 32) {       // whole warps; lanes past the end have a digit of their own
-      const bool in = i < hi;
-      const unsigned digit = in ? (key_at(i) >> shift) & (bins - 1) : none;
-      const unsigned peers = __match_any_sync(0xffffffffu, digit);
-      if (in && lane == __ffs(peers) - 1) mine[digit] += __popc(peers);
-      __syncwarp();
+    for (long long base = lo; base < hi; base += 32 * kKeys) {
+      unsigned key[kKeys];
+#pragma unroll
+      for (int k = 0; k < kKeys; ++k) key[k] = base + k * 32 + lane < hi ? key_at(base + k * 32 + lane) : 0;
+#pragma unroll
+      for (int k = 0; k < kKeys; ++k) {                            // whole warps; lanes past the end have a digit of their own
+        const bool in = base + k * 32 + lane < hi;
+        const unsigned digit = in ? (key[k] >> shift) & (bins - 1) : none;
+        const unsigned peers = __match_any_sync(0xffffffffu, digit);
+        if (in && lane == __ffs(peers) - 1) mine[digit] += __popc(peers);
+        __syncwarp();
+      }
     }
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += kSortThreads) {      // counts -> tokens of this digit in warps before; totals
@@ -221,18 +233,27 @@ embed_sort_fill_kernel(const ID* __restrict__ ids, const Sort s, uint4* __restri
     for (int w = 0; w < warp; ++w) below += sums[w];
     if (threadIdx.x < bins) bases[threadIdx.x] = below + scan - all + before;
     __syncthreads();
-    for (long long i = lo + lane; i < hi + lane; i += 32) {
-      const bool in = i < hi;
-      const unsigned key = in ? key_at(i) : none, digit = in ? (key >> shift) & (bins - 1) : none;
-      const unsigned pos = in && pass > 0 ? __ldcg(pos_in + i) : static_cast<unsigned>(i);
-      const unsigned peers = __match_any_sync(0xffffffffu, digit);
-      const unsigned at = in ? bases[digit] + mine[digit] + __popc(peers & ((1u << lane) - 1)) : 0;
-      __syncwarp();
-      if (in && lane == __ffs(peers) - 1) mine[digit] += __popc(peers);
-      __syncwarp();
-      if (in) {
-        key_out[at] = key;
-        pos_out[at] = pos;
+    for (long long base = lo; base < hi; base += 32 * kKeys) {
+      unsigned key[kKeys], pos[kKeys];
+#pragma unroll
+      for (int k = 0; k < kKeys; ++k) {
+        const long long i = base + k * 32 + lane;
+        key[k] = i < hi ? key_at(i) : 0;
+        pos[k] = i < hi && pass > 0 ? __ldcg(pos_in + i) : static_cast<unsigned>(i);
+      }
+#pragma unroll
+      for (int k = 0; k < kKeys; ++k) {
+        const bool in = base + k * 32 + lane < hi;
+        const unsigned digit = in ? (key[k] >> shift) & (bins - 1) : none;
+        const unsigned peers = __match_any_sync(0xffffffffu, digit);
+        const unsigned at = in ? bases[digit] + mine[digit] + __popc(peers & ((1u << lane) - 1)) : 0;
+        __syncwarp();
+        if (in && lane == __ffs(peers) - 1) mine[digit] += __popc(peers);
+        __syncwarp();
+        if (in) {
+          key_out[at] = key[k];
+          pos_out[at] = pos[k];
+        }
       }
     }
     __threadfence();
@@ -262,7 +283,7 @@ embed_sum_kernel(const unsigned* __restrict__ keys, const unsigned* __restrict__
   __syncthreads();
   const int col = blockIdx.y * kSlice + (VEC ? threadIdx.x * kCols : threadIdx.x);
   if (col >= d) return;
-  constexpr int kAhead = 4;
+  constexpr int kAhead = VEC && sizeof(T) == 2 ? 8 : 4;            // rows in flight
   float acc[kCols] = {};
   bool from_before = key_s[1] == key_s[0];
   for (int base = 0; base < count; base += kAhead) {
@@ -294,9 +315,10 @@ embed_sum_kernel(const unsigned* __restrict__ keys, const unsigned* __restrict__
   }
 }
 
-// Runs that begin in a window and go on: tail of that window, heads of the windows up to the run's end.
+// Runs that begin in a window and go on: tail of that window, then heads of the windows up to the run's end.  A CTA takes 256
+// columns, four to a thread; its four groups of 64 threads share the run's windows, and their sums are added in order.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kJoinThreads)
+__global__ void __launch_bounds__(kThreads)
 embed_join_kernel(const unsigned* __restrict__ keys, long long n, int window, long long v, int d, float scale,
                   const float* __restrict__ head, const float* __restrict__ tail, T* __restrict__ dw) {
   griddep_wait();
@@ -306,34 +328,48 @@ embed_join_kernel(const unsigned* __restrict__ keys, long long n, int window, lo
   const unsigned key = keys[next - 1];
   if (key >= v || keys[next] != key) return;                       // no run goes on
   if (keys[first] == key && w > 0 && keys[first - 1] == key) return;   // it began before
-  long long lo = next + 1, hi = n;                                 // the run's end: the first key above
-  while (lo < hi) {
-    const long long mid = (lo + hi) >> 1;
-    if (keys[mid] == key) lo = mid + 1;
-    else hi = mid;
-  }
-  const long long last = (lo - 1) / window;
-  for (int j = 0; j < (VEC ? 1 : 4); ++j) {
-    const int col = blockIdx.y * kJoinSlice + (VEC ? threadIdx.x * 4 : threadIdx.x + j * kJoinThreads);
-    if (col >= d) return;
-    if constexpr (VEC) {
-      float4 acc = *reinterpret_cast<const float4*>(tail + w * d + col);
-#pragma unroll 8
-      for (long long u = w + 1; u <= last; ++u) {
-        const float4 h = *reinterpret_cast<const float4*>(head + u * d + col);
-        acc.x += h.x; acc.y += h.y; acc.z += h.z; acc.w += h.w;
-      }
-      T* to = dw + key * static_cast<long long>(d) + col;
-      put(to, acc.x * scale);
-      put(to + 1, acc.y * scale);
-      put(to + 2, acc.z * scale);
-      put(to + 3, acc.w * scale);
-    } else {
-      float acc = tail[w * d + col];
-#pragma unroll 8
-      for (long long u = w + 1; u <= last; ++u) acc += head[u * d + col];
-      put(dw + key * static_cast<long long>(d) + col, acc * scale);
+  // The last window that the run reaches: each thread asks one window whether the run goes on behind it.
+  __shared__ int stop;
+  long long last = w + 1;
+  for (;; last += kThreads) {
+    const long long end = (last + threadIdx.x + 1) * window;       // first token behind the window
+    const bool goes_on = end < n && keys[end - 1] == key && keys[end] == key;
+    if (threadIdx.x == 0) stop = kThreads;
+    __syncthreads();
+    if (!goes_on) atomicMin(&stop, static_cast<int>(threadIdx.x));
+    __syncthreads();
+    const int at = stop;
+    __syncthreads();
+    if (at < kThreads) {
+      last += at;
+      break;
     }
+  }
+  auto load = [&](const float* row, int col) {
+    if constexpr (VEC) return *reinterpret_cast<const float4*>(row + col);
+    return make_float4(row[col], col + 1 < d ? row[col + 1] : 0.f, col + 2 < d ? row[col + 2] : 0.f, col + 3 < d ? row[col + 3] : 0.f);
+  };
+  auto add = [](float4& a, float4 b) { a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w; };
+  __shared__ float4 parts[kThreads];
+  const int group = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int col = blockIdx.y * kJoinSlice + lane * 4;
+  const long long each = (last - w + 3) / 4, lo = w + 1 + group * each, hi = min(lo + each, last + 1);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (col < d) {
+    if (group == 0) acc = load(tail + w * d, col);
+#pragma unroll 8
+    for (long long u = lo; u < hi; ++u) add(acc, load(head + u * d, col));
+  }
+  parts[threadIdx.x] = acc;
+  __syncthreads();
+  if (group == 0 && col < d) {
+#pragma unroll
+    for (int g = 1; g < 4; ++g) add(acc, parts[g * 64 + lane]);
+    T* to = dw + key * static_cast<long long>(d) + col;
+    put(to, acc.x * scale);
+    if (VEC || col + 1 < d) put(to + 1, acc.y * scale);
+    if (VEC || col + 2 < d) put(to + 2, acc.z * scale);
+    if (VEC || col + 3 < d) put(to + 3, acc.w * scale);
   }
 }
 
@@ -343,11 +379,12 @@ struct Plan {
   size_t list, partials;                     // bytes of one list of n entries, of head or of tail
 };
 
-// Windows: short enough that about four CTAs an SM have one, between 8 and 64 tokens (a longer one leaves fewer partial sums).
+// Windows: short enough that about two CTAs an SM have one, between 8 and 64 tokens.  Longer ones leave fewer partial sums, and the
+// longest run's are a chain: 16384 tokens of 4096 columns, a tenth of them one id, take 254 us in all with 32 and 246 with 64.
 Plan plan_of(long long n, int d, long long v) {
   Plan p;
   p.slices = static_cast<int>(ceil_div(d, kSlice));
-  const long long fit = n * p.slices / (4ll * sm_count());
+  const long long fit = n * p.slices / (2ll * sm_count());
   p.window = 8;
   while (p.window < 64 && p.window * 2 <= fit) p.window *= 2;
   p.windows = ceil_div(n, p.window);
@@ -392,10 +429,12 @@ template <typename ID>
 int launch_sort(const b200tp_embedding_args* a, const Sort& s, void* dw, cudaStream_t stream, int* status) {
   const long long bytes = a->v * a->d * (a->dtype == B200TP_BF16 ? 2 : 4);
   const size_t smem = static_cast<size_t>(kSortWarps + 2) * (size_t{4} << s.digit);
-  B200TP_CUDA_OK(cudaFuncSetAttribute(embed_sort_fill_kernel<ID>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  const long long blocks = kCluster + ceil_div(ceil_div(bytes, kFillBytes), kCluster) * kCluster;
-  B200TP_CUDA_OK(launch_pdl(embed_sort_fill_kernel<ID>, dim3(static_cast<unsigned>(blocks)), dim3(kSortThreads), smem, stream,
-                            static_cast<const ID*>(a->ids), s, static_cast<uint4*>(dw), bytes, status));
+  if (smem > 48 << 10)
+    B200TP_CUDA_OK(cudaFuncSetAttribute(embed_sort_kernel<ID>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  B200TP_CUDA_OK(launch_pdl(embed_sort_kernel<ID>, dim3(kCluster), dim3(kSortThreads), smem, stream, static_cast<const ID*>(a->ids), s,
+                            status));
+  B200TP_CUDA_OK(launch_pdl(embed_fill_kernel, dim3(static_cast<unsigned>(ceil_div(bytes, kFillBytes))), dim3(kSortThreads), 0, stream,
+                            static_cast<uint4*>(dw), static_cast<long long>(bytes)));
   return B200TP_OK;
 }
 
@@ -412,7 +451,7 @@ int launch_sums(const b200tp_embedding_args* a, const Plan& p, const unsigned* k
   if (p.windows == 1) return B200TP_OK;
   const dim3 join_grid(static_cast<unsigned>(p.windows), static_cast<unsigned>(ceil_div(a->d, kJoinSlice)));
   auto join = [&](auto kernel) {
-    return launch_pdl(kernel, join_grid, dim3(kJoinThreads), 0, stream, keys, a->n, p.window, a->v, a->d, a->scale, head, tail,
+    return launch_pdl(kernel, join_grid, dim3(kThreads), 0, stream, keys, a->n, p.window, a->v, a->d, a->scale, head, tail,
                       static_cast<T*>(dw));
   };
   B200TP_CUDA_OK(vec ? join(embed_join_kernel<T, true>) : join(embed_join_kernel<T, false>));

@@ -205,7 +205,7 @@ __device__ __forceinline__ Part joined(const Part* parts, const Tokens& t, long 
 // One block: a sequence's parts to a thread, then the batch's sums.  512 sequences of two parts: 32 kB.
 __global__ void __launch_bounds__(kJoinThreads)
 policy_join_kernel(const Part* __restrict__ parts, const Tokens t, int normalize, float* __restrict__ weights,
-                   float* __restrict__ out3) {
+                   float* __restrict__ loss_out, float* __restrict__ stats) {
   griddep_wait();
   griddep_launch_dependents();
   __shared__ double sums[kJoinThreads / 32];
@@ -230,9 +230,9 @@ policy_join_kernel(const Part* __restrict__ parts, const Tokens t, int normalize
   if (threadIdx.x == 0) {
     const double per = 1. / max(count, 1.);
     if (normalize != B200TP_NORMALIZE_SEQUENCE) weights[0] = normalize == B200TP_NORMALIZE_TOKEN ? static_cast<float>(per) : 1.f;
-    out3[0] = static_cast<float>(normalize == B200TP_NORMALIZE_TOKEN ? loss * per : loss);
-    out3[1] = static_cast<float>(kl * per);
-    out3[2] = static_cast<float>(clipped * per);
+    *loss_out = static_cast<float>(normalize == B200TP_NORMALIZE_TOKEN ? loss * per : loss);
+    stats[0] = static_cast<float>(kl * per);
+    stats[1] = static_cast<float>(clipped * per);
   }
 }
 
@@ -464,7 +464,7 @@ int b200tp_preference_loss_fwd(const b200tp_objective_args* a, int32_t kind, dou
 }
 
 int b200tp_policy_loss_fwd(const b200tp_objective_args* a, double clip_low, double clip_high, double kl_coef, int32_t kl_kind,
-                           int32_t normalize, float* out3, float* slopes, float* weights, void* workspace,
+                           int32_t normalize, float* loss, float* stats, float* slopes, float* weights, void* workspace,
                            size_t workspace_bytes, void* stream_v) {
   int rc = check(a);
   if (rc) return rc;
@@ -474,7 +474,7 @@ int b200tp_policy_loss_fwd(const b200tp_objective_args* a, double clip_low, doub
   if (normalize < B200TP_NORMALIZE_TOKEN || normalize > B200TP_NORMALIZE_SUM)
     return fail(B200TP_ERR_LOSS_INPUT, "unknown normalisation");
   if (kl_coef != 0. && a->ref_logps == nullptr && a->length > 0) return fail(B200TP_ERR_LOSS_INPUT, "a KL term needs ref_logps");
-  if (out3 == nullptr || weights == nullptr) return fail(B200TP_ERR_LOSS_INPUT, "null output");
+  if (loss == nullptr || stats == nullptr || weights == nullptr) return fail(B200TP_ERR_LOSS_INPUT, "null output");
   if (a->length > 0 && (a->old_logps == nullptr || a->advantages == nullptr))
     return fail(B200TP_ERR_LOSS_INPUT, "old_logps / advantages is null");
   rc = check_workspace(a, workspace, workspace_bytes);
@@ -499,7 +499,7 @@ int b200tp_policy_loss_fwd(const b200tp_objective_args* a, double clip_low, doub
                                        : launch_policy<float, float>(a, t, r, slopes, parts, stream);
   if (rc) return rc;
   B200TP_CUDA_OK(launch_pdl(policy_join_kernel, dim3(1), dim3(kJoinThreads), 0, stream, static_cast<const Part*>(parts), t, normalize,
-                            weights, out3));
+                            weights, loss, stats));
   return B200TP_OK;
 }
 

@@ -339,6 +339,21 @@ def test_no_gradient_wanted_and_second_derivative(cuda_device):
         torch.autograd.grad(loss, leaf, create_graph=True)
 
 
+def test_results_can_be_written_to(cuda_device):
+    """`loss /= n` for accumulated batches, and statistics scaled in place: the gradient is that of the scaled loss."""
+    x, o, r, _, _, _ = (t if t is None or not isinstance(t, torch.Tensor) else t.to(cuda_device) for t in _tokens(2, 64, False, torch.float32, 22))
+    a = torch.ones(2, 1, device=cuda_device)
+    for call in (lambda t: policy_loss(t, o, a, ref_logps=r, kl_coef=0.1), lambda t: preference_loss(t, r)):
+        leaf = x.clone().requires_grad_(True)
+        want, = torch.autograd.grad(call(leaf).loss * 0.25, leaf)
+        out = call(leaf)
+        loss = out.loss
+        loss /= 4
+        out[1].mul_(7.0)
+        out[2].zero_()
+        assert torch.equal(torch.autograd.grad(loss, leaf)[0], want)
+
+
 def test_saved_tensors_moved_to_the_host_and_back(cuda_device):
     """Hooks that keep what the backward needs on the host: the gradient is formed from what comes back."""
     x, o, r, mask, _, _ = _tokens(4, 200, False, torch.float32, 23)

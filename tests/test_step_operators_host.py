@@ -34,7 +34,7 @@ def test_objective_arguments(lib, change, text):
     assert lib.b200tp_objective_workspace_bytes(C.byref(a)) == 0
     assert text in lib.b200tp_last_error()
     assert lib.b200tp_preference_loss_fwd(C.byref(a), 0, 0.1, 0.0, 0.0, 0, PTR, PTR, PTR, PTR, 1 << 20, None) == _lib.ERR_LOSS_INPUT
-    assert lib.b200tp_policy_loss_fwd(C.byref(a), 0.2, 0.2, 0.0, 2, 0, PTR, PTR, PTR, PTR, 1 << 20, None) == _lib.ERR_LOSS_INPUT
+    assert lib.b200tp_policy_loss_fwd(C.byref(a), 0.2, 0.2, 0.0, 2, 0, PTR, PTR, PTR, PTR, PTR, 1 << 20, None) == _lib.ERR_LOSS_INPUT
     assert lib.b200tp_objective_bwd(C.byref(a), None, PTR, 1, PTR, PTR, None) == _lib.ERR_LOSS_INPUT
 
 
@@ -48,7 +48,7 @@ def test_objective_rules_and_workspace(lib):
     assert pref(a, beta=0.0) == _lib.ERR_LOSS_INPUT and pref(a, beta=float("nan")) == _lib.ERR_LOSS_INPUT and pref(a, loss=None) == _lib.ERR_LOSS_INPUT
     assert pref(a, ws=None) == _lib.ERR_WORKSPACE and pref(a, ws=PTR + 8) == _lib.ERR_WORKSPACE and pref(a, n=need - 1) == _lib.ERR_WORKSPACE
     pol = lambda a, low=0.2, high=0.2, coef=0.1, kl=2, norm=0: lib.b200tp_policy_loss_fwd(
-        C.byref(a), low, high, coef, kl, norm, PTR, PTR, PTR, PTR, need, None)
+        C.byref(a), low, high, coef, kl, norm, PTR, PTR, PTR, PTR, PTR, need, None)
     for bad in (dict(low=-0.1), dict(low=1.1), dict(high=-1.0), dict(kl=3), dict(norm=3), dict(norm=-1), dict(low=float("nan"))):
         assert pol(a, **bad) == _lib.ERR_LOSS_INPUT, bad
     assert pol(_objective(ref_logps=None)) == _lib.ERR_LOSS_INPUT and b"KL term" in lib.b200tp_last_error()
