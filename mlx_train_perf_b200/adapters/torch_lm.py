@@ -7,6 +7,10 @@ Both loss functions walk the inner model layer by layer --
 a `PackedMask` (a top-level `model(input_ids)` call would hand the blocks a tensor mask, which
 the flash wrapper refuses), then feed the hidden states to the fused loss with the logits never
 materialised.  Masked mean: loss = sum(nll * mask) / ntoks, reduced inside the library.
+
+`make_token_loss_fn` stops before that reduction; `make_preference_loss_fn` and `make_policy_loss_fn` go on from the
+per-token losses with the objectives of `core/objectives.py`.  Where the embedding table is trained, the walk looks rows
+up with `embedding_lookup`, whose gradient adds the rows of equal ids in a fixed order.
 """
 from __future__ import annotations
 
@@ -16,8 +20,10 @@ import torch
 
 from mlx_train_perf_b200.attention.segments import PackedMask
 from mlx_train_perf_b200.attention.wrapper import SUPPORTED_FAMILIES, FlashAttentionWrapper
-from mlx_train_perf_b200.core.loss import (IGNORE_INDEX, DenseHead, HeadRef, QuantizedHead,
+from mlx_train_perf_b200.core.embedding import embedding_lookup
+from mlx_train_perf_b200.core.loss import (IGNORE_INDEX, DenseHead, HeadRef, QuantizedHead, fused_linear_ce,
                                            reduced_linear_cross_entropy, resolve_impl, tied_head)
+from mlx_train_perf_b200.core.objectives import PolicyLoss, PreferenceLoss, policy_loss, preference_loss
 from mlx_train_perf_b200.errors import AdapterError
 
 
@@ -56,8 +62,25 @@ def split_model(model: Any) -> tuple[Callable[[torch.Tensor], torch.Tensor], Hea
     return trunk, head
 
 
+def _trains_plain_table(mod: Any) -> bool:
+    """Whether `embed_tokens` is a plain nn.Embedding with a trained fp32 / bf16 table on a GPU and nothing attached to it: then
+    `embedding_lookup` gives the same rows and the same gradient (summed in fp32, in token order, rounded once).  Anything
+    else (frozen, wrapped by an adapter, hooked, norm-limited, sparse) stays the module's own."""
+    if type(mod) is not torch.nn.Embedding or not torch.is_grad_enabled():
+        return False
+    w = mod.weight
+    return (isinstance(w, torch.Tensor) and w.is_cuda and w.requires_grad and w.dtype in (torch.float32, torch.bfloat16)
+            and mod.max_norm is None and not mod.sparse and not mod.scale_grad_by_freq
+            and not torch.is_autocast_enabled("cuda")
+            and not (mod._forward_hooks or mod._forward_pre_hooks or mod._backward_hooks or mod._backward_pre_hooks))
+
+
 def _walk(inner: Any, input_ids: torch.Tensor, mask: Any) -> torch.Tensor:
-    h = inner.embed_tokens(input_ids)
+    table = inner.embed_tokens
+    if _trains_plain_table(table) and input_ids.device == table.weight.device:
+        h = embedding_lookup(input_ids, table.weight, padding_idx=table.padding_idx)
+    else:
+        h = table(input_ids)
     b, length = input_ids.shape
     pos = torch.arange(length, device=input_ids.device)[None].expand(b, -1)   # never reset per segment
     rope = inner.rotary_emb(h, pos) if hasattr(inner, "rotary_emb") else None
@@ -74,6 +97,15 @@ def _require_wrapped(model: Any, who: str) -> None:
                                f"{type(layer.self_attn).__name__!r}")
 
 
+def _supervised(batch: torch.Tensor, lengths: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(mask, targets) of a (B, L+1) batch: position s (1-based, on the target axis) counts iff offset <= s <= length; the others'
+    targets are the ignored index."""
+    targets = batch[:, 1:]
+    steps = torch.arange(1, targets.shape[1] + 1, device=targets.device)
+    mask = (steps >= lengths[:, 0:1]) & (steps <= lengths[:, 1:2])
+    return mask, torch.where(mask, targets.to(torch.int64), torch.full_like(targets, IGNORE_INDEX, dtype=torch.int64))
+
+
 def make_loss_fn(model: Any, *, impl: str = "auto"):
     """`loss(model, batch, lengths) -> (loss, ntoks)`: batch int (B, L+1); lengths int (B, 2)
     = (offset, length) per row; position s (1-based, on the target axis) is supervised iff
@@ -83,18 +115,57 @@ def make_loss_fn(model: Any, *, impl: str = "auto"):
 
     def loss_fn(model_arg: Any, batch: torch.Tensor, lengths: torch.Tensor):
         trunk, head = split_model(model_arg)
-        inputs, targets = batch[:, :-1], batch[:, 1:]
-        hidden = trunk(inputs)
+        hidden = trunk(batch[:, :-1])
         resolve_impl(head=head, dtype=hidden.dtype, n=hidden.shape[0] * hidden.shape[1], d=hidden.shape[-1],
                      impl=impl)
-        steps = torch.arange(1, targets.shape[1] + 1, device=targets.device)
-        mask = (steps >= lengths[:, 0:1]) & (steps <= lengths[:, 1:2])
-        masked_targets = torch.where(mask, targets.to(torch.int64), torch.full_like(targets, IGNORE_INDEX,
-                                                                                     dtype=torch.int64))
+        _, masked_targets = _supervised(batch, lengths)
         # the masked mean (and the token count) are formed inside the library: unsupervised positions carry
         # ignore_index, so loss = sum(nll over supervised positions) / ntoks
         loss, count = reduced_linear_cross_entropy(hidden, head, masked_targets, impl=impl, reduction="mean")
         return loss, count.to(torch.int64)
+
+    return loss_fn
+
+
+def make_token_loss_fn(model: Any, *, impl: str = "auto"):
+    """`loss(model, batch, lengths) -> (nll, mask)`, (B, L) each: the per-token losses -log p of the targets and which positions are
+    supervised (the others' are 0); batch and lengths as in `make_loss_fn`.  Under `torch.no_grad()` this is the pass of a reference or
+    a sampling model."""
+    split_model(model)
+    _require_wrapped(model, "make_token_loss_fn")
+
+    def loss_fn(model_arg: Any, batch: torch.Tensor, lengths: torch.Tensor):
+        trunk, head = split_model(model_arg)
+        hidden = trunk(batch[:, :-1])
+        mask, masked_targets = _supervised(batch, lengths)
+        return fused_linear_ce(hidden, head, masked_targets, impl=impl)[0], mask
+
+    return loss_fn
+
+
+def make_preference_loss_fn(model: Any, *, impl: str = "auto", **rule):
+    """`loss(model, batch, lengths, ref_nll=None) -> PreferenceLoss`: rows [0, P) of the batch hold the chosen sequences, rows
+    [P, 2P) the rejected ones; `ref_nll` (B, L): the reference model's `make_token_loss_fn` losses.  `rule`: the keywords of
+    `preference_loss` (kind, beta, label_smoothing, margin, average)."""
+    token_losses = make_token_loss_fn(model, impl=impl)
+
+    def loss_fn(model_arg: Any, batch: torch.Tensor, lengths: torch.Tensor, ref_nll: torch.Tensor | None = None) -> PreferenceLoss:
+        nll, mask = token_losses(model_arg, batch, lengths)
+        return preference_loss(nll, ref_nll, mask=mask, from_nll=True, **rule)
+
+    return loss_fn
+
+
+def make_policy_loss_fn(model: Any, *, impl: str = "auto", **rule):
+    """`loss(model, batch, lengths, old_nll, advantages, ref_nll=None) -> PolicyLoss`: `old_nll`, `ref_nll` (B, L) the sampling and the
+    reference model's `make_token_loss_fn` losses, `advantages` (B, L) or (B, 1).  `rule`: the keywords of `policy_loss` (clip_low,
+    clip_high, kl_coef, kl, normalize)."""
+    token_losses = make_token_loss_fn(model, impl=impl)
+
+    def loss_fn(model_arg: Any, batch: torch.Tensor, lengths: torch.Tensor, old_nll: torch.Tensor, advantages: torch.Tensor,
+                ref_nll: torch.Tensor | None = None) -> PolicyLoss:
+        nll, mask = token_losses(model_arg, batch, lengths)
+        return policy_loss(nll, old_nll, advantages, ref_logps=ref_nll, mask=mask, from_nll=True, **rule)
 
     return loss_fn
 

@@ -68,6 +68,7 @@ class TrainConfig:
     grad_checkpoint: bool
     impl: str
     attention: str = "stock"
+    optimizer_bits: int = 32       # of AdamW's moments: 32, or 8 (codes and a pair of fp32 scales for every 256)
 
 
 @dataclass(frozen=True)
@@ -112,7 +113,13 @@ def _lora_bytes(cfg: TrainConfig, shape: ModelShape) -> int:
 
 
 def _optimizer_bytes(cfg: TrainConfig, shape: ModelShape, calib: Calibration) -> int:
-    return int(calib.optimizer_bytes_per_param * _lora_params(cfg, shape))
+    if cfg.optimizer_bits == 32:
+        per_param = calib.optimizer_bytes_per_param
+    elif cfg.optimizer_bits == 8:
+        per_param = 2 + 8 / 256
+    else:
+        raise PlanInputError(f"optimizer_bits must be 8 or 32, got {cfg.optimizer_bits}")
+    return int(per_param * _lora_params(cfg, shape))
 
 
 def _activation_bytes(cfg: TrainConfig, shape: ModelShape, calib: Calibration) -> int:

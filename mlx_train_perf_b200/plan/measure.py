@@ -4,7 +4,7 @@
 
 Builds a random-init Llama-shaped model (no checkpoint needed), freezes it, attaches rank-8 LoRA
 adapters to q_proj / v_proj of every layer (the planner's adapter model: two modules, two
-matrices), and runs AdamW train steps through the fused linear-cross-entropy loss at a grid of
+matrices), and runs this package's AdamW train steps through the fused linear-cross-entropy loss at a grid of
 sequence lengths with the stock (materialising) attention and with `enable_flash_attention`,
 checkpointed and not.  Each point records the MARGINAL peak -- `torch.cuda.max_memory_allocated`
 above what was resident when only the frozen weights were loaded -- and
@@ -24,6 +24,7 @@ from torch import nn
 from mlx_train_perf_b200.adapters.torch_lm import split_model
 from mlx_train_perf_b200.attention.wrapper import enable_flash_attention
 from mlx_train_perf_b200.core.loss import DenseHead, linear_cross_entropy
+from mlx_train_perf_b200.core.optim import AdamW
 from mlx_train_perf_b200.plan import estimate as E
 from mlx_train_perf_b200.plan.calibration import Calibration, load_calibration
 
@@ -79,7 +80,7 @@ def measure_point(cfg_kw: dict, shape: E.ModelShape, cfg: E.TrainConfig, device,
     if cfg.grad_checkpoint:
         m.gradient_checkpointing_enable(gradient_checkpointing_kwargs={"use_reentrant": False})
     m.train()
-    opt = torch.optim.AdamW(params, lr=1e-4)
+    opt = AdamW(params, lr=1e-4, bits=cfg.optimizer_bits)
     head = DenseHead(weight=m.lm_head.weight, trainable=False)
     if cfg.attention == "flash":
         trunk, _ = split_model(m)                                        # walks the wrapped layers, causal mask
