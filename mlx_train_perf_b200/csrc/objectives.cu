@@ -46,9 +46,7 @@ struct PolicyRule {
 
 // What a block knows of one sequence's share of tokens.
 struct alignas(32) Part {
-  double loss, kl;
-  int count, clipped;
-  double pad;
+  double loss, kl, count, clipped;
 };
 
 __device__ __forceinline__ float ld(const float* p) { return *p; }
@@ -61,40 +59,50 @@ __device__ __forceinline__ long long border(const Tokens& t, long long s) {
   return min(max(b, 0ll), t.length);
 }
 // Tokens [lo, hi) of block (s, k); borders that do not rise give empty sequences, never an access outside.
-__device__ __forceinline__ void share(const Tokens& t, long long s, int k, long long& lo, long long& hi) {
+__device__ __forceinline__ void share(const Tokens& t, long long s, int k, int& lo, int& hi) {
   lo = 0;
-  hi = t.length;
+  hi = static_cast<int>(t.length);                                  // at most 2^30
   if (t.cu != nullptr) {
-    lo = border(t, s);
-    hi = max(border(t, s + 1), lo);
+    lo = static_cast<int>(border(t, s));
+    hi = max(static_cast<int>(border(t, s + 1)), lo);
   }
-  const long long per = (hi - lo + t.splits - 1) / t.splits;
-  lo = min(lo + per * k, hi);
+  const int per = (hi - lo + t.splits - 1) / t.splits;
+  lo = static_cast<int>(min(lo + static_cast<long long>(per) * k, static_cast<long long>(hi)));
   hi = min(lo + per, hi);
 }
 
-__device__ __forceinline__ bool taken(const Tokens& t, long long s, long long i) {
-  return t.mask == nullptr || t.mask[s * t.mask_stride + i] != 0;
+// Sums of up to four values over a block of N threads, in a fixed order; all threads get them.
+template <int N, int K>
+__device__ __forceinline__ void block_sums(double (&v)[K], double (*shared)[K]) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  if ((threadIdx.x & 31) == 0)
+#pragma unroll
+    for (int k = 0; k < K; ++k) shared[threadIdx.x >> 5][k] = v[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    v[k] = (threadIdx.x & 31) < N / 32 ? shared[threadIdx.x & 31][k] : 0.;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  }
 }
 
-template <int N, typename T>
-__device__ __forceinline__ T block_sum(T v, T* shared) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-  __syncthreads();
-  T sum = 0;
-#pragma unroll
-  for (int w = 0; w < N / 32; ++w) sum += shared[w];
-  return sum;
-}
-
-// exp(z) - 1 - z without the cancellation near zero: below a quarter the Taylor series to z^9 / 9!, whose first term left out
-// is 2 z^8 / 10! < 1e-11 of the sum.
-__device__ __forceinline__ float exp_minus_line(float z, float expm1_z) {
-  if (fabsf(z) >= 0.25f) return expm1_z - z;
-  float s = 1.f / 362880.f;
+// exp(z) - 1 - z and exp(z) - 1 without cancellation: up to |z| = 1 the Taylor series to z^13 / 13!, whose first term left out
+// is 2 z^12 / 14! < 3e-11 of the sum; beyond, the library's expm1.  (Log ratios of a few tenths then leave hardly a warp with both
+// branches: 4 M tokens take 24 us, with the series up to 1/2 26.)
+__device__ __forceinline__ float exp_minus_line(float z, float* minus_one) {
+  if (fabsf(z) > 1.f) {
+    *minus_one = expm1f(z);
+    return *minus_one - z;
+  }
+  float s = 1.f / 6227020800.f;
+  s = fmaf(s, z, 1.f / 479001600.f);
+  s = fmaf(s, z, 1.f / 39916800.f);
+  s = fmaf(s, z, 1.f / 3628800.f);
+  s = fmaf(s, z, 1.f / 362880.f);
   s = fmaf(s, z, 1.f / 40320.f);
   s = fmaf(s, z, 1.f / 5040.f);
   s = fmaf(s, z, 1.f / 720.f);
@@ -102,7 +110,9 @@ __device__ __forceinline__ float exp_minus_line(float z, float expm1_z) {
   s = fmaf(s, z, 1.f / 24.f);
   s = fmaf(s, z, 1.f / 6.f);
   s = fmaf(s, z, 0.5f);
-  return s * z * z;
+  s *= z * z;
+  *minus_one = z + s;
+  return s;
 }
 
 // Per token:  u = x - o, ratio = exp(u);  clipped iff A > 0 and u > log(1 + high), or A < 0 and u < log(1 - low), which is
@@ -117,8 +127,7 @@ policy_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ old, const
                      Part* __restrict__ parts) {
   griddep_wait();
   griddep_launch_dependents();
-  __shared__ double sums[kThreads / 32];
-  __shared__ int counts[kThreads / 32];
+  __shared__ double sums[kThreads / 32][4];
   const long long s = blockIdx.x / t.splits;
   const int k = static_cast<int>(blockIdx.x % t.splits);
   const long long out_stride = t.cu != nullptr ? 0 : t.length;
@@ -130,27 +139,34 @@ policy_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ old, const
     }
     return;
   }
-  long long lo, hi;
+  int lo, hi;
   share(t, s, k, lo, hi);
+  // rows, so that the loop indexes with 32 bits (126 instructions a token with 64)
+  const TX* x_row = x + s * t.x_stride;
+  const TR* old_row = old + s * t.old_stride;
+  const TR* ref_row = REF ? ref + s * t.ref_stride : nullptr;
+  const float* adv_row = adv + s * t.adv_seq;
+  const unsigned char* mask_row = t.mask == nullptr ? nullptr : t.mask + s * t.mask_stride;
+  float* slope_row = slopes == nullptr ? nullptr : slopes + s * out_stride;
+  const bool adv_each = t.adv_tok != 0;
+  const float adv_one = adv_each || lo >= hi ? 0.f : adv_row[0];
   double loss = 0., kl_sum = 0.;
   int count = 0, clips = 0;
-  for (long long base = lo + threadIdx.x; base < hi; base += kThreads * kUnroll) {
+  for (int base = lo + threadIdx.x; base < hi; base += kThreads * kUnroll) {
     float xv[kUnroll], ov[kUnroll], rv[kUnroll], av[kUnroll];
     bool on[kUnroll];
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
-      const long long i = base + j * kThreads;
-      const bool in = i < hi;
-      const long long c = in ? i : lo;
-      on[j] = in && taken(t, s, c);
-      xv[j] = ld(x + s * t.x_stride + c);
-      ov[j] = ld(old + s * t.old_stride + c);
-      if constexpr (REF) rv[j] = ld(ref + s * t.ref_stride + c);
-      av[j] = adv[s * t.adv_seq + c * t.adv_tok];
+      const int i = base + j * kThreads, c = i < hi ? i : base;
+      on[j] = mask_row == nullptr || mask_row[c] != 0;
+      xv[j] = ld(x_row + c);
+      ov[j] = ld(old_row + c);
+      if constexpr (REF) rv[j] = ld(ref_row + c);
+      av[j] = adv_each ? adv_row[c * t.adv_tok] : adv_one;
     }
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
-      const long long i = base + j * kThreads;
+      const int i = base + j * kThreads;
       if (i >= hi) break;
       float slope = 0.f;
       if (on[j]) {
@@ -163,9 +179,8 @@ policy_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ old, const
           const float z = t.sign * (rv[j] - xv[j]);
           float kl_slope;
           if (r.kl_kind == B200TP_KL_K3) {
-            const float e = expm1f(z);
-            kl = exp_minus_line(z, e);
-            kl_slope = -e;
+            kl = exp_minus_line(z, &kl_slope);
+            kl_slope = -kl_slope;
           } else if (r.kl_kind == B200TP_KL_K2) {
             kl = 0.5f * z * z;
             kl_slope = -z;
@@ -180,18 +195,17 @@ policy_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ old, const
         count += 1;
         clips += clipped;
       }
-      if (slopes != nullptr) slopes[s * out_stride + i] = t.sign * slope;
+      if (slope_row != nullptr) slope_row[i] = t.sign * slope;
     }
   }
-  loss = block_sum<kThreads>(loss, sums);
-  if constexpr (REF) kl_sum = block_sum<kThreads>(kl_sum, sums);
-  count = block_sum<kThreads>(count, counts);
-  clips = block_sum<kThreads>(clips, counts);
-  if (threadIdx.x == 0) parts[blockIdx.x] = Part{loss, kl_sum, count, clips, 0.};
+  double all[4] = {loss, kl_sum, static_cast<double>(count), static_cast<double>(clips)};       // counts are exact
+  block_sums<kThreads>(all, sums);
+  if (threadIdx.x == 0) parts[blockIdx.x] = Part{all[0], all[1], all[2], all[3]};
 }
 
+// A sequence's parts joined.  Up to eight: each thread of the warp does its own sequence `s`.  More: the warp's lanes share one.
 __device__ __forceinline__ Part joined(const Part* parts, const Tokens& t, long long s) {
-  Part p{0., 0., 0, 0, 0.};
+  Part p{0., 0., 0., 0.};
   for (int k = 0; k < t.splits; ++k) {
     const Part q = parts[s * t.splits + k];
     p.loss += q.loss;
@@ -201,32 +215,50 @@ __device__ __forceinline__ Part joined(const Part* parts, const Tokens& t, long 
   }
   return p;
 }
+__device__ __forceinline__ Part joined_by_warp(const Part* parts, const Tokens& t, long long s) {
+  double v[4] = {0., 0., 0., 0.};
+#pragma unroll 4
+  for (int k = threadIdx.x & 31; k < t.splits; k += 32) {
+    const Part q = parts[s * t.splits + k];
+    v[0] += q.loss;
+    v[1] += q.kl;
+    v[2] += q.count;
+    v[3] += q.clipped;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  return Part{v[0], v[1], v[2], v[3]};
+}
+constexpr int kFewParts = 8;
 
-// One block: a sequence's parts to a thread, then the batch's sums.  512 sequences of two parts: 32 kB.
+// One block: the sequences' sums, then the batch's.
 __global__ void __launch_bounds__(kJoinThreads)
 policy_join_kernel(const Part* __restrict__ parts, const Tokens t, int normalize, float* __restrict__ weights,
                    float* __restrict__ loss_out, float* __restrict__ stats) {
   griddep_wait();
   griddep_launch_dependents();
-  __shared__ double sums[kJoinThreads / 32];
-  double loss = 0., kl = 0., count = 0., clipped = 0.;      // counts in double: exact to 2^53
-  for (long long s = threadIdx.x; s < t.seqs; s += kJoinThreads) {
-    const Part p = joined(parts, t, s);
+  __shared__ double sums[kJoinThreads / 32][4];
+  double all[4] = {0., 0., 0., 0.};           // loss, kl, taken and clipped tokens
+  const bool few = t.splits <= kFewParts;
+  const int step = few ? kJoinThreads : kJoinThreads / 32;
+  for (long long s = few ? threadIdx.x : threadIdx.x >> 5; s < t.seqs; s += step) {
+    const Part p = few ? joined(parts, t, s) : joined_by_warp(parts, t, s);
+    if (!few && (threadIdx.x & 31) != 0) continue;
     double l = p.loss;
     if (normalize == B200TP_NORMALIZE_SEQUENCE) {
-      const double w = 1. / (static_cast<double>(t.seqs) * max(p.count, 1));
+      const double w = 1. / (static_cast<double>(t.seqs) * max(p.count, 1.));
       l *= w;
       weights[s] = static_cast<float>(w);
     }
-    loss += l;
-    kl += p.kl;
-    count += p.count;
-    clipped += p.clipped;
+    all[0] += l;
+    all[1] += p.kl;
+    all[2] += p.count;
+    all[3] += p.clipped;
   }
-  loss = block_sum<kJoinThreads>(loss, sums);
-  kl = block_sum<kJoinThreads>(kl, sums);
-  count = block_sum<kJoinThreads>(count, sums);
-  clipped = block_sum<kJoinThreads>(clipped, sums);
+  block_sums<kJoinThreads>(all, sums);
+  const double loss = all[0], kl = all[1], count = all[2], clipped = all[3];
   if (threadIdx.x == 0) {
     const double per = 1. / max(count, 1.);
     if (normalize != B200TP_NORMALIZE_SEQUENCE) weights[0] = normalize == B200TP_NORMALIZE_TOKEN ? static_cast<float>(per) : 1.f;
@@ -242,23 +274,24 @@ __global__ void __launch_bounds__(kThreads)
 preference_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ ref, const Tokens t, Part* __restrict__ parts) {
   griddep_wait();
   griddep_launch_dependents();
-  __shared__ double sums[kThreads / 32];
-  __shared__ int counts[kThreads / 32];
+  __shared__ double sums[kThreads / 32][2];
   const long long s = blockIdx.x / t.splits;
-  long long lo, hi;
+  int lo, hi;
   share(t, s, static_cast<int>(blockIdx.x % t.splits), lo, hi);
+  const TX* x_row = x + s * t.x_stride;
+  const TR* ref_row = REF ? ref + s * t.ref_stride : nullptr;
+  const unsigned char* mask_row = t.mask == nullptr ? nullptr : t.mask + s * t.mask_stride;
   double sum = 0.;
   int count = 0;
-  for (long long base = lo + threadIdx.x; base < hi; base += kThreads * kUnroll) {
+  for (int base = lo + threadIdx.x; base < hi; base += kThreads * kUnroll) {
     float xv[kUnroll], rv[kUnroll];
     bool on[kUnroll];
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
-      const long long i = base + j * kThreads;
-      const long long c = i < hi ? i : lo;
-      on[j] = i < hi && taken(t, s, c);
-      xv[j] = ld(x + s * t.x_stride + c);
-      if constexpr (REF) rv[j] = ld(ref + s * t.ref_stride + c);
+      const int i = base + j * kThreads, c = i < hi ? i : base;
+      on[j] = i < hi && (mask_row == nullptr || mask_row[c] != 0);
+      xv[j] = ld(x_row + c);
+      if constexpr (REF) rv[j] = ld(ref_row + c);
     }
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
@@ -269,9 +302,9 @@ preference_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ ref, c
       count += 1;
     }
   }
-  sum = block_sum<kThreads>(sum, sums);
-  count = block_sum<kThreads>(count, counts);
-  if (threadIdx.x == 0) parts[blockIdx.x] = Part{sum * t.sign, 0., count, 0, 0.};
+  double all[2] = {sum * t.sign, static_cast<double>(count)};
+  block_sums<kThreads>(all, sums);
+  if (threadIdx.x == 0) parts[blockIdx.x] = Part{all[0], 0., all[1], 0.};
 }
 
 // One block: pair i is the sequences i and P + i.  h = beta (l_i - l_{P + i}) - margin; out: the loss, the S rewards
@@ -281,12 +314,16 @@ preference_join_kernel(const Part* __restrict__ parts, const Tokens t, int kind,
                        int average, float* __restrict__ loss_out, float* __restrict__ rewards, float* __restrict__ weights) {
   griddep_wait();
   griddep_launch_dependents();
-  __shared__ double sums[kJoinThreads / 32];
+  __shared__ double sums[kJoinThreads / 32][1];
   const long long pairs = t.seqs / 2;
   double total = 0.;
-  for (long long i = threadIdx.x; i < pairs; i += kJoinThreads) {
-    const Part c = joined(parts, t, i), r = joined(parts, t, pairs + i);
-    const double cs = average ? 1. / max(c.count, 1) : 1., rs = average ? 1. / max(r.count, 1) : 1.;
+  const bool few = t.splits <= kFewParts;
+  const int step = few ? kJoinThreads : kJoinThreads / 32;
+  for (long long i = few ? threadIdx.x : threadIdx.x >> 5; i < pairs; i += step) {
+    const Part c = few ? joined(parts, t, i) : joined_by_warp(parts, t, i);
+    const Part r = few ? joined(parts, t, pairs + i) : joined_by_warp(parts, t, pairs + i);
+    if (!few && (threadIdx.x & 31) != 0) continue;
+    const double cs = average ? 1. / max(c.count, 1.) : 1., rs = average ? 1. / max(r.count, 1.) : 1.;
     const double lc = c.loss * cs, lr = r.loss * rs;
     const double h = beta * (lc - lr) - margin;
     double f, slope;
@@ -310,8 +347,9 @@ preference_join_kernel(const Part* __restrict__ parts, const Tokens t, int kind,
     rewards[i] = static_cast<float>(beta * lc);
     rewards[pairs + i] = static_cast<float>(beta * lr);
   }
-  total = block_sum<kJoinThreads>(total, sums);
-  if (threadIdx.x == 0) *loss_out = static_cast<float>(total / static_cast<double>(pairs));
+  double all[1] = {total};
+  block_sums<kJoinThreads>(all, sums);
+  if (threadIdx.x == 0) *loss_out = static_cast<float>(all[0] / static_cast<double>(pairs));
 }
 
 // grad = upstream * weight * (slopes ? slope : mask).  `per_seq`: a weight for each sequence, else one.
@@ -332,32 +370,35 @@ objective_grad_kernel(const float* __restrict__ slopes, const float* __restrict_
     }
     return;
   }
-  long long lo, hi;
+  int lo, hi;
   share(t, s, k, lo, hi);
+  const unsigned char* mask_row = t.mask == nullptr ? nullptr : t.mask + s * t.mask_stride;
+  const float* slope_row = SLOPES ? slopes + s * out_stride : nullptr;
+  TX* grad_row = grad + s * out_stride;
   const float w = *upstream * weights[per_seq ? s : 0];
-  for (long long base = lo + threadIdx.x; base < hi; base += kThreads * kUnroll) {
+  for (int base = lo + threadIdx.x; base < hi; base += kThreads * kUnroll) {
     float v[kUnroll];
     bool on[kUnroll];
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
-      const long long i = base + j * kThreads;
-      const long long c = i < hi ? i : lo;
-      on[j] = taken(t, s, c);
-      v[j] = SLOPES ? slopes[s * out_stride + c] : 1.f;
+      const int i = base + j * kThreads, c = i < hi ? i : base;
+      on[j] = mask_row == nullptr || mask_row[c] != 0;
+      v[j] = SLOPES ? slope_row[c] : 1.f;
     }
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
-      const long long i = base + j * kThreads;
-      if (i < hi) st(grad + s * out_stride + i, on[j] ? w * v[j] : 0.f);
+      const int i = base + j * kThreads;
+      if (i < hi) st(grad_row + i, on[j] ? w * v[j] : 0.f);
     }
   }
 }
 
-// Blocks a sequence: about 2048 tokens each on average, at most eight blocks an SM in all and at most 512 a sequence.
+// Blocks a sequence: about 1024 tokens each on average (one round of loads a thread), at most eight blocks an SM in all and at most
+// 512 a sequence.
 int splits_of(long long seqs, long long length, bool packed) {
   const int64_t mean = packed ? ceil_div(length, seqs) : length;
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(512, 8ll * sm_count() / seqs));
-  return static_cast<int>(std::max<int64_t>(1, std::min(most, ceil_div(mean, 2048))));
+  return static_cast<int>(std::max<int64_t>(1, std::min(most, ceil_div(mean, kThreads * kUnroll))));
 }
 
 int check(const b200tp_objective_args* a) {
