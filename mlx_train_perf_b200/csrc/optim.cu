@@ -39,6 +39,7 @@ constexpr int kRound = 4096;                // elements that a CTA loads at once
 template <int BITS>
 constexpr int kChunk = BITS == 8 ? kRound : 2 * kRound;
 constexpr int kTensors = 600;               // of one launch: 26 kB of its parameters
+constexpr int kNear = 64;                   // entries of the coarse index
 constexpr int kFew = 48;                    // of the small form: 2 kB
 
 struct Rule {
@@ -71,7 +72,8 @@ struct Table {
   long long numel[N];
   long long at[N];                          // of the tensor's first element in the states
   int first[N + 1];                         // chunk of the tensor's first element
-  int count;
+  short near[kNear + 1];                    // the tensor of chunk k << shift, the last one behind the end
+  int shift;
 };
 
 template <typename T>
@@ -157,6 +159,13 @@ __device__ __forceinline__ float rcp_ftz(float v) {
   return q;
 }
 
+// 448 / v, with a Newton step behind the approximate reciprocal: all codes of a block depend on it.
+__device__ __forceinline__ float over(float v) {
+  const float q = rcp_ftz(v);
+  return 448.f * fmaf(fmaf(-v, q, 1.f), q, q);
+}
+constexpr float kNoRoot = 4e-19f;           // roots up to here stand for zero: the root of 1e-37 is 3.2e-19
+
 // Two e4m3 codes of a word, the lower or the upper ones.
 __device__ __forceinline__ Pair decode2(uint32_t w, int upper) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(upper ? w >> 16 : w & 0xffffu), __NV_E4M3);
@@ -172,12 +181,11 @@ __device__ __forceinline__ uint32_t mix(uint32_t pair, uint32_t step) {
   return x ^ (x >> 16);
 }
 
-// y >= 0 to the e4m3 value below or above, up with a probability of the distance (dither uniform in [0, 2^20)); not zero unless y
-// is.  Below 2^-6, where e4m3 values lie 2^-9 apart, 2^-6 is added first: sums in [2^-6, 2^-5) lie as far apart.
+// y > 0 to the e4m3 value below or above, up with a probability of the distance (dither uniform in [0, 2^20)); never zero.  Below 2^-6, where e4m3 values lie 2^-9 apart, 2^-6 is added first: sums in [2^-6, 2^-5) lie as far apart.
 __device__ __forceinline__ float dithered(float y, uint32_t dither) {
   const float lift = y < 0x1p-6f ? 0x1p-6f : 0.f;
   const uint32_t u = __float_as_uint(y + lift) + dither;
-  return fmaxf(__uint_as_float(u & 0xfff00000u) - lift, y > 0.f ? 0x1p-9f : 0.f);
+  return fmaxf(__uint_as_float(u & 0xfff00000u) - lift, 0x1p-9f);
 }
 
 // Eight elements as they lie in memory.
@@ -211,7 +219,8 @@ __device__ __forceinline__ void unpack(const Raw8<float>& r, Pair (&v)[4]) {
 
 // 8-bit moments of eight elements: (codes, scales) and gradients in, parameters moved, (codes, scales) out.
 // m = beta1 sm code + one_beta1 g;  v = (sqrt(beta2) sv code)^2 + (sqrt(one_beta2) g)^2, g times grad_scale;  sqrt(v) from v rsqrt(v) and
-// one Newton step (about an ulp; a v below 1e-37 counts as that small a one: its root is 0 or far below eps).
+// one Newton step (about an ulp).  1e-37 is added to v, which keeps rsqrt finite and changes no v above 1e-30; what is then below
+// 1.6e-37 is zero.
 __device__ __forceinline__ void step8(uint2& mc, uint2& vc, float2& sc, const Pair (&g)[4], Pair (&p)[4], float grad_scale,
                                       const Rule& r, uint32_t position) {
   Pair m[4], root[4];
@@ -224,16 +233,15 @@ __device__ __forceinline__ void step8(uint2& mc, uint2& vc, float2& sc, const Pa
     const Pair cm = decode2(i < 2 ? mc.x : mc.y, i & 1), cv = decode2(i < 2 ? vc.x : vc.y, i & 1);
     m[i] = fma2(g[i], gm, mul2(cm, bm));
     const Pair new_root = mul2(g[i], gr), old_root = mul2(cv, bv);
-    const Pair v = fma2(new_root, new_root, mul2(old_root, old_root));
-    const Pair q = Pair{rsqrt_ftz(fmaxf(v.x, 1e-37f)), rsqrt_ftz(fmaxf(v.y, 1e-37f))};
+    const Pair v = fma2(new_root, new_root, fma2(old_root, old_root, both(1e-37f)));
+    const Pair q = Pair{rsqrt_ftz(v.x), rsqrt_ftz(v.y)};
     const Pair t = mul2(v, q);
     root[i] = fma2(Pair{fmaf(-t.x, t.x, v.x), fmaf(-t.y, t.y, v.y)}, mul2(q, both(0.5f)), t);
     const Pair d = fma2(root[i], both(r.root), both(r.eps));
     const Pair move = mul2(m[i], Pair{rcp_ftz(d.x), rcp_ftz(d.y)});
     p[i] = fma2(move, both(-r.rate), mul2(p[i], both(r.decay)));
     ma = fmaxf(ma, fmaxf(fabsf(m[i].x), fabsf(m[i].y)));
-    const Pair either = fma2(m[i], both(0.f), root[i]);             // the root, or NaN where either is not finite
-    top = max(top, max(__float_as_uint(either.x), __float_as_uint(either.y)));
+    top = max(top, max(__float_as_uint(root[i].x), __float_as_uint(root[i].y)));     // a gradient that voids m voids v too
   }
   top = __reduce_max_sync(0xffffffffu, top);                        // by their bits: what is not finite lies above all else
   const bool finite = top < 0x7f800000u;
@@ -253,10 +261,12 @@ __device__ __forceinline__ void step8(uint2& mc, uint2& vc, float2& sc, const Pa
     }
     top = __reduce_max_sync(0xffffffffu, top);
   }
-  const float mm = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(ma))), rm = __uint_as_float(top);
-  // moments of 1e-30 and less are zero: their scale's reciprocal would overflow (a root is 0 or above 1e-23)
-  const Pair mi = both(mm > 1e-30f ? 448.f * rcp_ftz(mm) : 0.f), ri = both(rm > 0.f ? 448.f * rcp_ftz(rm) : 0.f);
-  sc = make_float2(mm > 1e-30f ? mm * (1.f / 448.f) : 0.f, rm * (1.f / 448.f));
+  // moments of 1e-30 and less are zero: their scale's reciprocal would overflow
+  float mm = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(ma))), rm = __uint_as_float(top);
+  mm = mm > 1e-30f ? mm : 0.f;
+  rm = rm > kNoRoot ? rm : 0.f;
+  const Pair mi = both(mm > 0.f ? over(mm) : 0.f), ri = both(rm > 0.f ? over(rm) : 0.f);
+  sc = make_float2(mm * (1.f / 448.f), rm * (1.f / 448.f));
   uint32_t mw[4], vw[4], low = 0xffffffffu;
   Pair y[4];
 #pragma unroll
@@ -284,7 +294,8 @@ __device__ __forceinline__ void step8(uint2& mc, uint2& vc, float2& sc, const Pa
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t bits = mix(pair + i, r.step);
-      float a = dithered(y[i].x, ((bits & 0xffffu) << 4) | 8u), b = dithered(y[i].y, ((bits >> 16) << 4) | 8u);
+      float a = root[i].x > kNoRoot ? dithered(y[i].x, ((bits & 0xffffu) << 4) | 8u) : 0.f;
+      float b = root[i].y > kNoRoot ? dithered(y[i].y, ((bits >> 16) << 4) | 8u) : 0.f;
       if (isnan(root[i].x)) a = NAN;
       if (isnan(root[i].y)) b = NAN;
       vw[i] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
@@ -298,9 +309,10 @@ __global__ void __launch_bounds__(kThreads, 4)
 adamw_kernel(const __grid_constant__ Table<N> table, const States st, const Rule r) {
   griddep_wait();
   griddep_launch_dependents();
-  // the tensor of this chunk: the last one whose first chunk is not beyond it
+  // The tensor of this chunk: the last one whose first chunk is not beyond it, from a coarse index and a search between two of its
+  // entries (each step waits for the one before; one warp searching for all, behind a barrier, cost 8 %).
   const int chunk = blockIdx.x;
-  int lo = 0, hi = table.count - 1;
+  int lo = table.near[chunk >> table.shift], hi = table.near[(chunk >> table.shift) + 1];
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (table.first[mid] <= chunk) lo = mid;
@@ -411,7 +423,12 @@ int launch_n(const b200tp_adamw_tensor* t, int count, const States& st, const Ru
   }
   if (kept == 0) return B200TP_OK;
   table.first[kept] = chunks;
-  table.count = kept;
+  table.shift = 0;
+  while (((chunks - 1) >> table.shift) >= kNear) ++table.shift;
+  for (int k = 0, i = 0; k <= kNear; ++k) {
+    while (i + 1 < kept && table.first[i + 1] <= static_cast<int64_t>(k) << table.shift) ++i;
+    table.near[k] = static_cast<short>(i);
+  }
   B200TP_CUDA_OK(launch_pdl(adamw_kernel<TP, TG, BITS, MASTER, N>, dim3(chunks), dim3(kThreads), 0, stream, table, st, r));
   return B200TP_OK;
 }
