@@ -17,6 +17,7 @@ from __future__ import annotations
 from typing import Any, Callable
 
 import torch
+from torch.nn.modules.module import _has_any_global_hook
 
 from mlx_train_perf_b200.attention.segments import PackedMask
 from mlx_train_perf_b200.attention.wrapper import SUPPORTED_FAMILIES, FlashAttentionWrapper
@@ -66,7 +67,7 @@ def _trains_plain_table(mod: Any) -> bool:
     """Whether `embed_tokens` is a plain nn.Embedding with a trained fp32 / bf16 table on a GPU and nothing attached to it: then
     `embedding_lookup` gives the same rows and the same gradient (summed in fp32, in token order, rounded once).  Anything
     else (frozen, wrapped by an adapter, hooked, norm-limited, sparse) stays the module's own."""
-    if type(mod) is not torch.nn.Embedding or not torch.is_grad_enabled():
+    if type(mod) is not torch.nn.Embedding or not torch.is_grad_enabled() or _has_any_global_hook():
         return False
     w = mod.weight
     return (isinstance(w, torch.Tensor) and w.is_cuda and w.requires_grad and w.dtype in (torch.float32, torch.bfloat16)

@@ -58,9 +58,9 @@ class _Lookup(torch.autograd.Function):
         grad = torch.empty((v, d), dtype=dtype, device=dev)
         a = _lib.EmbeddingArgs(ids.data_ptr(), ids.numel(), v, d, dtype is torch.bfloat16, ids.dtype is torch.int64, scale, rows.stride(0),
                                padding)
-        nbytes = lib.b200tp_embedding_bwd_workspace_bytes(C.byref(a))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         with _lib.on(dev):
+            nbytes = lib.b200tp_embedding_bwd_workspace_bytes(C.byref(a))     # goes by the device's SMs
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             rc = lib.b200tp_embedding_bwd(C.byref(a), rows.data_ptr(), grad.data_ptr(), ws.data_ptr(), nbytes, _lib.stream(dev),
                                           device_status(dev).data_ptr())
         _lib.check(rc)

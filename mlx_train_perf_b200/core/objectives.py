@@ -113,7 +113,8 @@ class _Call:
     def buffer(self, lib, a, logps, slopes: bool) -> tuple[torch.Tensor, int, int, int]:
         """One allocation for the workspace, the weights of sequences or of the batch, and the tokens' slopes: (buffer, workspace bytes,
         address of the weights, address of the slopes or 0)."""
-        nbytes = lib.b200tp_objective_workspace_bytes(C.byref(a))
+        with _lib.on(logps.device):                       # the blocks go by that device's SMs
+            nbytes = lib.b200tp_objective_workspace_bytes(C.byref(a))
         self.at = nbytes // 4
         count = self.seqs if self.per_sequence else 1
         buf = torch.empty(self.at + count + (logps.numel() if slopes else 0), dtype=torch.float32, device=logps.device)

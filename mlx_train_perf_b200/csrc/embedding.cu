@@ -40,6 +40,11 @@ __device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162floa
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// An id outside the table; a word that is already there stays.
+__device__ __forceinline__ void report(int* status) {
+  if (status != nullptr) atomicCAS(status, 0, B200TP_DEV_BAD_INDEX);
+}
+
 // Eight columns of a row.  VEC: adjacent ones from `col`, 16-byte loads; else `col + j * step`, those below d.
 template <typename T, bool VEC>
 struct Cols {
@@ -116,7 +121,7 @@ embed_fwd_kernel(const ID* __restrict__ ids, const T* __restrict__ weight, long 
   const int first = static_cast<int>(item - row * parts) * 1024;
   const long long id = static_cast<long long>(ids[row]);
   const bool ok = id >= 0 && id < v;
-  if (!ok && lane == 0 && status != nullptr) *status = B200TP_DEV_BAD_INDEX;
+  if (!ok && lane == 0) report(status);
   const T* from = weight + (ok ? id : 0) * w_stride;
   T* to = out + row * d;
   Cols<T, VEC> c[4];
@@ -182,7 +187,7 @@ embed_sort_kernel(const ID* __restrict__ ids, const Sort s, int* status) {
       if (pass > 0) return __ldcg(key_in + i);                    // written by other CTAs of the cluster
       const long long id = static_cast<long long>(ids[i]);
       if (id >= 0 && id < s.v) return static_cast<unsigned>(id == s.padding ? s.v : id);
-      if (status != nullptr) *status = B200TP_DEV_BAD_INDEX;
+      report(status);
       return static_cast<unsigned>(s.v);
     };
     for (int b = threadIdx.x; b < kSortWarps * bins; b += kSortThreads) counts[b] = 0;

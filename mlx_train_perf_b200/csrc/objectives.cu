@@ -188,10 +188,10 @@ policy_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ old, const
             kl = -z;
             kl_slope = 1.f;
           }
-          slope = fmaf(r.kl_coef, kl_slope, slope);
+          if (r.kl_coef != 0.f) slope = fmaf(r.kl_coef, kl_slope, slope);
           kl_sum += kl;
         }
-        loss += fmaf(r.kl_coef, kl, -gain);
+        loss += r.kl_coef != 0.f ? fmaf(r.kl_coef, kl, -gain) : -gain;     // an infinite KL that is only reported stays out
         count += 1;
         clips += clipped;
       }
@@ -329,7 +329,8 @@ preference_join_kernel(const Part* __restrict__ parts, const Tokens t, int kind,
     double f, slope;
     if (kind == B200TP_PREFERENCE_SIGMOID) {
       const double e = exp(-fabs(h)), tail = log1p(e);
-      f = (1. - smoothing) * (tail + max(-h, 0.)) + smoothing * (tail + max(h, 0.));
+      f = (1. - smoothing) * (tail + max(-h, 0.));
+      if (smoothing > 0.) f += smoothing * (tail + max(h, 0.));       // an infinite h must not meet a factor of zero
       slope = smoothing - (h >= 0. ? e : 1.) / (1. + e);             // smoothing - sigmoid(-h)
     } else if (kind == B200TP_PREFERENCE_HINGE) {
       f = h > 1. ? 0. : 1. - h;

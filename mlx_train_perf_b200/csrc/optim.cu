@@ -462,7 +462,8 @@ int launch_kind(const b200tp_adamw_args* a, const b200tp_adamw_tensor* t, int co
 
 bool misaligned(const void* p, unsigned mask) { return (reinterpret_cast<uintptr_t>(p) & mask) != 0; }
 
-// Two written ranges that overlap would race: the same tensor twice, or two views of one another.
+// Written ranges that overlap, or overlap what another tensor's step reads, would race: the same tensor twice, views of one another, an
+// output over another tensor's input.
 int check_apart(std::vector<std::pair<uintptr_t, uintptr_t>>& ranges, const char* what) {
   std::sort(ranges.begin(), ranges.end());
   for (size_t i = 1; i < ranges.size(); ++i)
@@ -490,7 +491,7 @@ int check(const b200tp_adamw_args* a, const b200tp_adamw_tensor* t, int32_t coun
   for (const void* p : states)
     if (misaligned(p, 15)) return fail(B200TP_ERR_OPTIM_INPUT, "states must be 16-byte aligned");
   std::vector<std::pair<uintptr_t, uintptr_t>> written, offsets;
-  written.reserve(count);
+  written.reserve(2 * count);
   offsets.reserve(count);
   const unsigned p_item = a->param_dtype == B200TP_BF16 ? 2 : 4, g_item = a->grad_dtype == B200TP_BF16 ? 2 : 4;
   for (int i = 0; i < count; ++i) {
@@ -501,8 +502,9 @@ int check(const b200tp_adamw_args* a, const b200tp_adamw_tensor* t, int32_t coun
       return fail(B200TP_ERR_OPTIM_INPUT, "a tensor is not aligned to its elements");
     if (t[i].state_offset < 0 || t[i].state_offset % kBlock != 0)
       return fail(B200TP_ERR_OPTIM_INPUT, "a tensor's place in the states must be a multiple of 256 elements");
-    const uintptr_t p = reinterpret_cast<uintptr_t>(t[i].param_out);
+    const uintptr_t p = reinterpret_cast<uintptr_t>(t[i].param_out), q = reinterpret_cast<uintptr_t>(t[i].param);
     written.emplace_back(p, p + static_cast<uintptr_t>(t[i].numel) * p_item);
+    if (q != p && a->master == nullptr) written.emplace_back(q, q + static_cast<uintptr_t>(t[i].numel) * p_item);   // read by others
     offsets.emplace_back(t[i].state_offset, t[i].state_offset + align_up(t[i].numel, kBlock));
   }
   const int rc = check_apart(written, "parameters");

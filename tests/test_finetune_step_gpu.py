@@ -135,6 +135,9 @@ def test_which_tables_the_walk_looks_up(cuda_device):
     hook = mod.register_forward_hook(lambda *a: None)
     assert not torch_lm._trains_plain_table(mod)
     hook.remove()
+    hook = torch.nn.modules.module.register_module_forward_hook(lambda *a: None)
+    assert not torch_lm._trains_plain_table(mod)
+    hook.remove()
     assert torch_lm._trains_plain_table(mod)
     for other in (torch.nn.Embedding(10, 8, max_norm=1.0), torch.nn.Embedding(10, 8, sparse=True), torch.nn.Embedding(10, 8, scale_grad_by_freq=True),
                   torch.nn.Embedding(10, 8).half(), torch.nn.Sequential(mod), torch.nn.Embedding(10, 8).requires_grad_(False)):

@@ -242,6 +242,23 @@ def test_values_that_count_and_are_not_finite_are_seen(cuda_device):
     assert math.isnan(policy_loss(x, torch.zeros_like(x), a).loss.item())
 
 
+def test_infinite_ratios_where_they_do_not_count(cuda_device):
+    """A rejected sequence that the model rules out is a loss of zero, not NaN; a KL term that is only reported may be infinite."""
+    x = torch.zeros(2, 4, device=cuda_device)
+    x[1, 2] = -math.inf
+    x.requires_grad_(True)
+    out = preference_loss(x, beta=0.3)
+    out.loss.backward()
+    assert out.loss.item() == 0.0 and (x.grad == 0).all() and out.rejected_rewards.item() == -math.inf
+    y = torch.zeros(2, 4, device=cuda_device, requires_grad=True)
+    r = torch.zeros(2, 4, device=cuda_device)
+    r[0, 1] = -math.inf
+    a = torch.ones(2, 1, device=cuda_device)
+    out = policy_loss(y, torch.zeros_like(r), a, ref_logps=r)
+    out.loss.backward()
+    assert out.loss.item() == -1.0 and out.kl.item() == math.inf and (y.grad == -0.125).all()
+
+
 def test_strided_rows_and_empty_masks(cuda_device):
     """Rows of a wider tensor (the usual shift by one), columns of a transposed one, expanded references; nothing counts at all."""
     dev = cuda_device

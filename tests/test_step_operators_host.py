@@ -84,7 +84,8 @@ def test_adamw_arguments(lib, change):
 @pytest.mark.parametrize("rows", [
     [[0, PTR, PTR, 100, 0]], [[PTR, 0, PTR, 100, 0]], [[PTR, PTR, 0, 100, 0]], [[PTR, PTR, PTR, -1, 0]], [[PTR, PTR, PTR, 100, 128]],
     [[PTR, PTR, PTR, 100, -256]], [[PTR + 1, PTR, PTR, 100, 0]], [[PTR, PTR + 2, PTR, 100, 0]],
-    [ROW, ROW], [ROW, [PTR, PTR, PTR + 396, 100, 256]], [ROW, [PTR, PTR, PTR + 400, 100, 0]], [[PTR, PTR, PTR, 257, 0], [PTR, PTR, PTR + 4096, 8, 256]]])
+    [ROW, ROW], [ROW, [PTR, PTR, PTR + 396, 100, 256]], [ROW, [PTR, PTR, PTR + 400, 100, 0]], [[PTR, PTR, PTR, 257, 0], [PTR, PTR, PTR + 4096, 8, 256]],
+    [[PTR, PTR, PTR + 8, 100, 0]], [[PTR, PTR, PTR + 4096, 100, 0], [PTR + 4196, PTR, PTR + 8192, 100, 256]]])
 def test_adamw_tables(lib, rows):
     assert _adamw(rows) == _lib.ERR_OPTIM_INPUT
 
