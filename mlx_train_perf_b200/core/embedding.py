@@ -60,9 +60,9 @@ class _Lookup(torch.autograd.Function):
                                padding)
         with _lib.on(dev):
             nbytes = lib.b200tp_embedding_bwd_workspace_bytes(C.byref(a))     # goes by the device's SMs
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            rc = lib.b200tp_embedding_bwd(C.byref(a), rows.data_ptr(), grad.data_ptr(), ws.data_ptr(), nbytes, _lib.stream(dev),
-                                          device_status(dev).data_ptr())
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+            rc = lib.b200tp_embedding_bwd(C.byref(a), rows.data_ptr(), grad.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
+                                          _lib.stream(dev), device_status(dev).data_ptr())
         _lib.check(rc)
         return grad, None, None, None
 

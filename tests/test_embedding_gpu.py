@@ -53,7 +53,9 @@ def _check_lookup(got, ids, w, scale):
 @pytest.mark.parametrize("n,v,d,kind", [
     (1, 1, 1, "uniform"), (1, 1000, 64, "uniform"), (7, 3, 5, "uniform"), (60, 32768, 1024, "words"), (31, 511, 8, "uniform"),
     (8, 512, 2048, "one"), (9, 512, 2056, "one"), (257, 513, 67, "words"), (1000, 40, 2049, "words"), (4096, 7, 96, "uniform"),
-    (16384, 151936, 128, "words"), (5000, 300000, 40, "uniform"), (70001, 1000, 72, "words"), (20000, 5, 520, "one"), (300, 70000, 4104, "uniform")])
+    (16384, 151936, 128, "words"), (5000, 300000, 40, "uniform"), (70001, 1000, 72, "words"), (20000, 5, 520, "one"), (300, 70000, 4104, "uniform"),
+    (256, 3000, 1024, "words"), (64, 9, 2056, "one"), (65, 9, 2056, "one"), (64, 20, 4100, "uniform"), (50, 70001, 67, "words"),
+    (64, 40, 16384, "words"), (64, 40, 16392, "words"), (33, 8, 3, "uniform")])
 def test_lookup_and_gradient(cuda_device, n, v, d, kind, dtype):
     dev = cuda_device
     g = torch.Generator().manual_seed(n + v)

@@ -95,7 +95,7 @@ def test_adamw_of_nothing(lib):
 
 
 def _embedding(**change):
-    a = _lib.EmbeddingArgs(PTR, 100, 1000, 64, 1, 1, 1.0, 64, -1)
+    a = _lib.EmbeddingArgs(PTR, 300, 1000, 64, 1, 1, 1.0, 64, -1)
     for k, v in change.items():
         setattr(a, k, v)
     return a
@@ -114,7 +114,8 @@ def test_embedding_pointers_and_workspace(lib):
     a = _embedding()
     need = lib.b200tp_embedding_bwd_workspace_bytes(C.byref(a))
     # keys and places twice, and two partial sums of a row for each window of 8 tokens at least
-    assert 16 * 100 <= need <= 4 * 512 + 2 * (13 * 64 * 4 + 256)
+    assert 16 * 300 <= need <= 4 * 1280 + 2 * (38 * 64 * 4 + 256)
+    assert lib.b200tp_embedding_bwd_workspace_bytes(C.byref(_embedding(n=64))) == 0       # up to 64 tokens: no sort
     bwd = lambda dy=PTR, dw=PTR, ws=PTR, n=need: lib.b200tp_embedding_bwd(C.byref(a), dy, dw, ws, n, None, None)
     assert bwd(dy=None) == bwd(dw=None) == bwd(dw=PTR + 8) == _lib.ERR_EMBEDDING_INPUT
     assert bwd(ws=None) == bwd(ws=PTR + 16) == bwd(n=need - 1) == _lib.ERR_WORKSPACE
