@@ -157,24 +157,16 @@ embed_direct_kernel(const ID* __restrict__ ids, int n, long long v, long long pa
   __shared__ unsigned match[kDirect / 32];
   const long long first = static_cast<long long>(blockIdx.x) * rows;
   const long long end = min(first + rows, v);
-  bool mine = false;
-  if (threadIdx.x < kDirect) {
-    long long id = -1;
-    if (threadIdx.x < n) {
-      id = static_cast<long long>(ids[threadIdx.x]);
-      if ((id < 0 || id >= v) && blockIdx.x == 0) report(status);
-    }
-    mine = id >= first && id < end && id != padding;
-    local[threadIdx.x] = mine ? static_cast<int>(id - first) : -1;
-  }
-  const bool any = __syncthreads_or(mine);
-  // rows are a multiple of eight, so that the CTA's share begins on a 16-byte boundary
+  const long long id = static_cast<int>(threadIdx.x) < n ? static_cast<long long>(ids[threadIdx.x]) : -1;    // n <= kDirect
+  // rows are a multiple of eight, so that the CTA's share begins on a 16-byte boundary; the id arrives meanwhile
   const long long bytes = (end - first) * d * static_cast<long long>(sizeof(T));
   uint4* fill = reinterpret_cast<uint4*>(dw + first * d);
   for (long long i = threadIdx.x; i < bytes / 16; i += kDirectThreads) fill[i] = make_uint4(0, 0, 0, 0);
   if (threadIdx.x < (bytes & 15) / 2) reinterpret_cast<unsigned short*>(fill)[bytes / 16 * 8 + threadIdx.x] = 0;
-  if (!any) return;
-  __syncthreads();
+  if (static_cast<int>(threadIdx.x) < n && (id < 0 || id >= v) && blockIdx.x == 0) report(status);
+  const bool mine = id >= first && id < end && id != padding;
+  if (threadIdx.x < kDirect) local[threadIdx.x] = mine ? static_cast<int>(id - first) : -1;
+  if (!__syncthreads_or(mine)) return;             // the barrier also puts the zeros before the sums
   for (int t = 0; t < n; ++t) {
     const int row = local[t];
     if (row < 0) continue;                         // the same for all threads
