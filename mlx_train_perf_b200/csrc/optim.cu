@@ -34,8 +34,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kBlock = 256;                 // elements that share a scale; tensors start at multiples of it in the states
 constexpr int kRound = 4096;                // elements that a CTA loads at once: two blocks a warp
-// Elements of one CTA.  8-bit moments: one round (94 % of the measured copy rate at 789 M elements; two rounds need either 120
-// registers, 75 %, or spills, 84 %).  32 bits: two, which halves the searches of the table (unaligned tensors: 100 % against 92 %).
+// Elements of one CTA.  8-bit moments: one round (two in a loop need 120 registers or spill: a quarter and a seventh slower at 789 M
+// elements).  32 bits: two, which halves the searches of the table (unaligned tensors: 100 % of the copy rate against 92 %).
 template <int BITS>
 constexpr int kChunk = BITS == 8 ? kRound : 2 * kRound;
 constexpr int kTensors = 600;               // of one launch: 26 kB of its parameters
