@@ -151,20 +151,21 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
     which, numels = range(len(params)), state.numels
     try:
         whole = all(map(_T.is_contiguous, grads))
-    except TypeError:                                    # a gradient is None
-        if out is not None:
-            raise OptimizerInputError("with out, every tensor needs a gradient") from None
+    except (TypeError, RuntimeError):                    # a gradient is None, or of a layout that has no such property
+        whole = False
+    if not whole:
         which = [i for i, g in enumerate(grads) if g is not None]
+        if len(which) < len(grads) and out is not None:
+            raise OptimizerInputError("with out, every tensor needs a gradient")
         if not which:
             return
-        rows = rows[which]
-        grads, numels = [grads[i] for i in which], tuple(numels[i] for i in which)
-        whole = False
+        rows, numels = rows[which], tuple(numels[i] for i in which)
+        if any(grads[i].layout is not torch.strided for i in which):
+            raise OptimizerInputError("gradients must be dense")
+        grads = [grads[i].contiguous() for i in which]
     g_dtype = grads[0].dtype
-    if g_dtype not in _DTYPES or grads[0].layout is not torch.strided:
-        raise OptimizerInputError(f"gradients must be dense and fp32 or bf16, got {g_dtype} {grads[0].layout}")
-    if not whole:
-        grads = [g.contiguous() for g in grads]
+    if g_dtype not in _DTYPES:
+        raise OptimizerInputError(f"gradients must be fp32 or bf16, got {g_dtype}")
     rows[:, 1] = _pointers("grads", grads, numels, g_dtype, dev, contiguous=True)
     scale_ptr = None
     if isinstance(grad_scale, torch.Tensor):

@@ -190,6 +190,20 @@ def test_tensors_without_gradients_and_of_different_ages(cuda_device):
     assert state.steps == [5, 4, 4] and all(torch.equal(p, q) for p, q in zip(params, single))
 
 
+def test_a_strided_gradient_before_a_missing_one(cuda_device):
+    dev = cuda_device
+    params = _tensors([(6, 50), (40,), (7, 9)], torch.float32, dev, 11)
+    same = [p.clone() for p in params]
+    g = _tensors([(50, 6), (40,), (9, 7)], torch.float32, dev, 12)
+    state, other = AdamWState.zeros(params), AdamWState.zeros(params)
+    adamw_step(params, [g[0].t(), None, g[2].t()], state, **RULE)
+    adamw_step(same, [g[0].t().contiguous(), g[1], g[2].t().contiguous()], other, **RULE)
+    assert torch.equal(params[0], same[0]) and torch.equal(params[2], same[2]) and not torch.equal(params[1], same[1])
+    assert state.steps == [1, 0, 1]
+    with pytest.raises(OptimizerInputError, match="dense"):
+        adamw_step(params[:2], [g[0].t(), g[1].to_sparse()], AdamWState.zeros(params[:2]), **RULE)
+
+
 def test_8_bit_roots_are_rounded_without_drift(cuda_device):
     """A million equal roots between two codes: the mean of the codes is the root, up to five standard errors and the dither's own
     2^-17 of a step; and a v that is not zero never becomes zero, whatever the block's largest."""
