@@ -30,7 +30,9 @@ class _Lookup(torch.autograd.Function):
         v, d = weight.shape
         dev, dtype = weight.device, weight.dtype
         rows = _rows(weight)
-        out = torch.empty((*ids.shape, d), dtype=dtype, device=dev)
+        shape = ids.shape
+        out = (torch.empty_strided((shape[0], d), (d, 1), dtype=dtype, device=dev) if len(shape) == 1
+               else torch.empty((*shape, d), dtype=dtype, device=dev))
         if not ids.is_contiguous():
             ids = ids.contiguous()
         a = _lib.EmbeddingArgs(ids.data_ptr(), ids.numel(), v, d, dtype is torch.bfloat16, ids.dtype is torch.int64, scale, rows.stride(0),
@@ -55,7 +57,7 @@ class _Lookup(torch.autograd.Function):
         if d_out.ndim != 2:
             d_out = d_out.reshape(-1, d)
         rows = _rows(d_out)
-        grad = torch.empty((v, d), dtype=dtype, device=dev)
+        grad = torch.empty_strided((v, d), (d, 1), dtype=dtype, device=dev)
         a = _lib.EmbeddingArgs(ids.data_ptr(), ids.numel(), v, d, dtype is torch.bfloat16, ids.dtype is torch.int64, scale, rows.stride(0),
                                padding)
         with _lib.on(dev):

