@@ -13,6 +13,7 @@ same per-token values.  Nothing here synchronises with the host unless `validate
 from __future__ import annotations
 
 import ctypes as C
+from functools import partial
 from typing import Literal, NamedTuple
 
 import torch
@@ -155,7 +156,8 @@ class _Call:
 
 
 class _Preference(torch.autograd.Function):
-    """logps -> loss; `call.out` gets the rewards.  Keeps a weight for each sequence."""
+    """logps -> loss; `call.out` gets the rewards.  Keeps a weight for each sequence.  Without a gradient `forward` is called by
+    itself (`ctx` None)."""
 
     @staticmethod
     def forward(ctx, logps, call):
@@ -240,7 +242,7 @@ def preference_loss(logps: torch.Tensor, ref_logps: torch.Tensor | None = None, 
     mask, ref = _check_mask(mask, logps), _check_other("ref_logps", ref_logps, logps)
     rule = (_PREFERENCES[kind], float(beta), float(label_smoothing), float(margin), bool(average))
     call = _call(logps, seqs, mask, cu_seqlens, None, ref, rule, from_nll, True)
-    loss = _Preference.apply(_unit_inner(logps), call)
+    loss = (_Preference.apply if call.recorded else partial(_Preference.forward, None))(_unit_inner(logps), call)
     return PreferenceLoss(loss, call.out[:seqs // 2], call.out[seqs // 2:])
 
 
@@ -283,5 +285,5 @@ def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor, advantages: torch.
     rule = (float(clip_low), float(clip_high), float(kl_coef), _KLS[kl], _NORMALIZE[normalize])
     call = _call(logps, seqs, mask, cu_seqlens, old, ref, rule, from_nll, normalize == "sequence")
     call.adv, call.adv_strides = adv, strides
-    loss = _Policy.apply(_unit_inner(logps), call)
+    loss = (_Policy.apply if call.recorded else partial(_Policy.forward, None))(_unit_inner(logps), call)
     return PolicyLoss(loss, *call.out)
