@@ -424,6 +424,13 @@ typedef struct b200tp_adamw_args {
  * launch.  Tensors that share memory are refused. */
 int b200tp_adamw_step(const b200tp_adamw_args* a, const b200tp_adamw_tensor* tensors, int32_t count, void* stream);
 
+/* Writes the addresses of `count` Python tensor objects into column 0 (param), 1 (grad) or 2 (param_out) of `rows`.  describe: the
+ * DLPack exchange table's dltensor_from_py_object_no_sync (header version 1.x) of the objects' own type; call with the
+ * interpreter's lock held.  -1: done; i >= 0: object i is not row-major, of `dtype`, on CUDA device `device` (-1: host) and of
+ * rows[i].numel elements; -2: `describe` failed and a Python exception is set. */
+int b200tp_tensor_rows(void* describe, const int64_t* objects, int32_t count, int32_t dtype, int32_t device,
+                       b200tp_adamw_tensor* rows, int32_t column);
+
 /* ---------------------------------------------------------------------------------------
  * Embedding lookup
  * ------------------------------------------------------------------------------------- */

@@ -8,6 +8,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import threading
+from functools import partial
 from pathlib import Path
 
 import torch
@@ -150,6 +151,7 @@ SIGNATURES = {
                                    C.c_size_t, C.c_void_p, C.c_void_p]),
     # the tensors: (count, 5) int64 rows param, grad, param_out, numel, state_offset
     "b200tp_adamw_step": (C.c_int, [C.POINTER(AdamwArgs), C.c_void_p, C.c_int32, C.c_void_p]),
+    "b200tp_tensor_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_int32]),
     "b200tp_embedding_fwd": (C.c_int, [C.POINTER(EmbeddingArgs), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "b200tp_embedding_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(EmbeddingArgs)]),
     "b200tp_embedding_bwd": (C.c_int, [C.POINTER(EmbeddingArgs), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p,
@@ -194,6 +196,30 @@ def load() -> C.CDLL:
             fn.argtypes = args
         _lib = lib
     return _lib
+
+
+_tensor_rows = None
+
+
+def tensor_rows():
+    """`(objects, count, dtype, device, rows, column) -> int`, b200tp_tensor_rows on torch tensors (see the header), or None where this
+    torch has no DLPack exchange table of version 1."""
+    global _tensor_rows
+    if _tensor_rows is None:
+        load()
+        _tensor_rows = False
+        capsule = getattr(torch.Tensor, "__dlpack_c_exchange_api__", None)
+        if capsule is not None:
+            get = C.pythonapi.PyCapsule_GetPointer
+            get.restype, get.argtypes = C.c_void_p, [C.py_object, C.c_char_p]
+            table = get(capsule, b"dlpack_exchange_api")
+            if C.c_uint32.from_address(table).value == 1:
+                # two words of header, then the allocator, two functions for owning exchange, and the one wanted here
+                describe = C.c_void_p.from_address(table + 5 * C.sizeof(C.c_void_p)).value
+                fn = C.PyDLL(str(LIB_PATH)).b200tp_tensor_rows            # keeps the interpreter's lock
+                fn.restype, fn.argtypes = SIGNATURES["b200tp_tensor_rows"]
+                _tensor_rows = partial(fn, describe)
+    return _tensor_rows or None
 
 
 _SAME_DEVICE = contextlib.nullcontext()

@@ -36,6 +36,7 @@ SOURCES = [
     "prestep.cu",
     "objectives.cu",
     "optim.cu",
+    "tensors.cu",
     "embedding.cu",
 ]
 

@@ -204,6 +204,31 @@ def test_a_strided_gradient_before_a_missing_one(cuda_device):
         adamw_step(params[:2], [g[0].t(), g[1].to_sparse()], AdamWState.zeros(params[:2]), **RULE)
 
 
+def test_tensors_asked_one_by_one(cuda_device, monkeypatch):
+    """Without the DLPack table (another torch), or with a tensor class of its own: the same step, the same refusals."""
+    from mlx_train_perf_b200 import _lib
+
+    class Own(torch.Tensor):
+        pass
+
+    dev = cuda_device
+    params, grads = _tensors([(6, 50), (40,)], torch.bfloat16, dev, 13), _tensors([(6, 50), (40,)], torch.bfloat16, dev, 14)
+    want = [p.clone() for p in params]
+    adamw_step(want, grads, AdamWState.zeros(want), **RULE)
+    own = [p.clone().as_subclass(Own) for p in params]
+    adamw_step(own, grads, AdamWState.zeros(own), **RULE)
+    assert all(torch.equal(a.as_subclass(torch.Tensor), b) for a, b in zip(own, want))
+    monkeypatch.setattr(_lib, "tensor_rows", lambda: None)
+    state = AdamWState.zeros(params)
+    for bad in ([grads[0], grads[1].float()], [grads[0], grads[1].cpu()], [grads[0], grads[1][:39]], [grads[0].half(), grads[1].half()]):
+        with pytest.raises(OptimizerInputError):
+            adamw_step(params, bad, state, **RULE)
+    with pytest.raises(OptimizerInputError):
+        adamw_step([params[0].t(), params[1]], grads, state, **RULE)
+    adamw_step(params, grads, state, **RULE)
+    assert all(torch.equal(a, b) for a, b in zip(params, want))
+
+
 def test_8_bit_roots_are_rounded_without_drift(cuda_device):
     """A million equal roots between two codes: the mean of the codes is the root, up to five standard errors and the dither's own
     2^-17 of a step; and a v that is not zero never becomes zero, whatever the block's largest."""

@@ -90,6 +90,32 @@ def test_adamw_tables(lib, rows):
     assert _adamw(rows) == _lib.ERR_OPTIM_INPUT
 
 
+def test_addresses_of_many_tensors(lib):
+    """The DLPack table of this torch, on host tensors: addresses of row-major tensors of the type and size, the first other one's index."""
+    fn = _lib.tensor_rows()
+    if fn is None:
+        pytest.skip("this torch has no DLPack exchange table")
+    good = [torch.zeros(3, 4), torch.nn.Parameter(torch.zeros(7)), torch.zeros(5)[2:], torch.zeros(0, 4), torch.zeros(()), torch.zeros(1, 6, 1),
+            torch.zeros(6, 2)[:, :1][:4].t()[:, :1]]
+    rows = np.zeros((len(good), 5), dtype=np.int64)
+    rows[:, 3] = [t.numel() for t in good]
+
+    def ask(tensors, dtype=0, device=-1, column=0):
+        return fn(np.fromiter(map(id, tensors), np.int64, len(tensors)).ctypes.data, len(tensors), dtype, device, rows.ctypes.data, column)
+
+    for column in (0, 1, 2):
+        assert ask(good, column=column) == -1
+        assert [p for p, t in zip(rows[:, column].tolist(), good) if t.numel()] == [t.data_ptr() for t in good if t.numel()]
+    assert ask(good, dtype=1) == 0 and ask(good, device=0) == 0 and ask(good, column=3) == len(good)
+    rows[:2, 3] = 12
+    for bad in (torch.zeros(4, 3).t(), torch.zeros(3, 4, dtype=torch.bfloat16), torch.zeros(3, 4, dtype=torch.int32), torch.zeros(13),
+                torch.zeros(3, 1).expand(3, 4), torch.zeros(24)[::2]):
+        assert ask([good[0], bad]) == 1
+    with pytest.raises(Exception):
+        ask([torch.zeros(12).to_sparse()])
+    assert ask([good[0].to(torch.bfloat16)], dtype=1) == -1
+
+
 def test_adamw_of_nothing(lib):
     assert _adamw([]) == _lib.OK
 
