@@ -220,9 +220,9 @@ __device__ __forceinline__ void unpack(const Raw8<float>& r, Pair (&v)[4]) {
 // 8-bit moments of eight elements: (codes, scales) and gradients in, parameters moved, (codes, scales) out.
 // m = beta1 sm code + one_beta1 g;  v = (sqrt(beta2) sv code)^2 + (sqrt(one_beta2) g)^2, g times grad_scale;  sqrt(v) from v rsqrt(v) and
 // one Newton step (about an ulp).  1e-37 is added to v, which keeps rsqrt finite and changes no v above 1e-30; what is then below
-// 1.6e-37 is zero.
+// 1.6e-37 is zero.  `pair`: half the first element's place in the states, which fixes the dither.
 __device__ __forceinline__ void step8(uint2& mc, uint2& vc, float2& sc, const Pair (&g)[4], Pair (&p)[4], float grad_scale,
-                                      const Rule& r, uint32_t position) {
+                                      const Rule& r, uint32_t pair) {
   Pair m[4], root[4];
   const Pair bm = both(r.beta1 * sc.x), bv = both(r.root_beta2 * sc.y);
   const Pair gm = both(r.one_beta1 * grad_scale), gr = both(r.root_one_beta2 * grad_scale);
@@ -277,7 +277,6 @@ __device__ __forceinline__ void step8(uint2& mc, uint2& vc, float2& sc, const Pa
     low = min(low, min(__float_as_uint(y[i].x), __float_as_uint(y[i].y)));
   }
   mc = make_uint2(mw[0] | (mw[1] << 16), mw[2] | (mw[3] << 16));
-  const uint32_t pair = position >> 1;
   if (finite && low >= 0x3c800000u) {
     // All of the thread's y lie at 2^-6 or above: a code is its fp32 bits 20 to 26 after the dither and less the exponents' distance
     // (120 << 23).  Times 16 they are the top byte: u * 16 + (dither * 16 - (120 << 27)), the latter put together from bytes.
@@ -366,7 +365,7 @@ adamw_kernel(const __grid_constant__ Table<N> table, const States st, const Rule
         Pair gv[4], pv[4];
         unpack(gr[it], gv);
         unpack(pr[it], pv);
-        step8(mc[it], vc[it], sc[it], gv, pv, grad_scale, r, static_cast<uint32_t>(j0) + it * kStep);
+        step8(mc[it], vc[it], sc[it], gv, pv, grad_scale, r, static_cast<uint32_t>(j0 >> 1) + it * (kStep / 2));
         const float flat[8] = {pv[0].x, pv[0].y, pv[1].x, pv[1].y, pv[2].x, pv[2].y, pv[3].x, pv[3].y};
         if constexpr (MASTER) store8(st.master_out + j0 + it * kStep, true, 8, flat);
         store8(op + it * kStep, whole || p_vec, mine(it), flat);

@@ -296,6 +296,26 @@ def test_what_is_not_finite_stays_by_itself(cuda_device):
         assert not torch.isfinite(got[0][2][bad]).any()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_offsets_beyond_32_bits(cuda_device, bits):
+    """A tensor of more than 2^31 elements and one behind it: the first step moves a weight by lr against its gradient's sign, whatever
+    the gradient's size, at both ends; the rest stays."""
+    dev = cuda_device
+    n = (1 << 31) + 300
+    params = [torch.zeros(n, dtype=torch.bfloat16, device=dev), torch.zeros(1000, dtype=torch.bfloat16, device=dev)]
+    grads = [torch.zeros_like(p) for p in params]
+    places = [0, 5, 1 << 30, n - 257, n - 1]
+    for k, at in enumerate(places):
+        grads[0][at] = 0.5 - k % 2
+    grads[1][[0, 999]] = -1.0
+    state = AdamWState.zeros(params, bits=bits)
+    adamw_step(params, grads, state, lr=0.25, weight_decay=0.0)
+    assert [params[0][at].item() for at in places] == [-0.25, 0.25, -0.25, 0.25, -0.25]
+    assert torch.count_nonzero(params[0]).item() == len(places) and params[1].tolist() == [0.25] + [0.0] * 998 + [0.25]
+    for k, at in enumerate(places):
+        assert state.exp_avg.float()[at].item() * (0.5 - k % 2) > 0 if bits == 8 else state.exp_avg[at].item() == pytest.approx(0.1 * (0.5 - k % 2))
+
+
 def test_tensors_that_share_memory_are_refused(cuda_device):
     dev = cuda_device
     p = torch.zeros(1000, device=dev)
