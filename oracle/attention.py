@@ -64,7 +64,8 @@ def flash_attention_reference(q, k, v, *, scale: float, causal: bool = True, seg
     lse = torch.logsumexp(s, dim=-1)
     p = torch.exp(s - lse[..., None])
     vg = _gather_kv(v.detach().cpu().to(dtype), q.shape[1], k.shape[1])
-    return p @ vg, lse
+    # by 32 columns: a host library may add in another order for another width, and columns must not depend on their neighbours
+    return torch.cat([p @ part for part in vg.split(32, dim=-1)], dim=-1), lse
 
 
 def math_attention(q, k, v, *, scale: float, causal: bool = True, seg_id=None,
