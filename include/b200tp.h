@@ -1,6 +1,7 @@
 /*
  * b200tp -- C ABI of the B200 (sm_100a) fused linear-cross-entropy and flash-attention
- * kernels.  One shared library, plain pointers and sizes, no framework types.
+ * kernels, and of the steps around them (embedding, objectives, AdamW).  One shared library, plain
+ * pointers and sizes, no framework types.
  *
  * Conventions
  *   - Every pointer is a caller-owned DEVICE pointer valid on `stream` unless stated.
@@ -450,8 +451,8 @@ typedef struct b200tp_embedding_args {
  * (adapters/mlx_lm.py:140-164). */
 int b200tp_embedding_fwd(const b200tp_embedding_args* a, const void* weight, void* out, void* stream, int* status);
 
-/* d_weight (v, d) contiguous, 16-byte aligned, every row written: scale times the sum, in the order of i and in f32, of d_out[i] over the
- * tokens with that id. */
+/* d_weight (v, d) contiguous, 16-byte aligned, every row written: scale times the sum of d_out[i] over the tokens with that id, in f32
+ * and in a fixed order. */
 size_t b200tp_embedding_bwd_workspace_bytes(const b200tp_embedding_args* a);
 int b200tp_embedding_bwd(const b200tp_embedding_args* a, const void* d_out, void* d_weight, void* workspace,
                          size_t workspace_bytes, void* stream, int* status);

@@ -65,7 +65,7 @@ def split_model(model: Any) -> tuple[Callable[[torch.Tensor], torch.Tensor], Hea
 
 def _trains_plain_table(mod: Any) -> bool:
     """Whether `embed_tokens` is a plain nn.Embedding with a trained fp32 / bf16 table on a GPU and nothing attached to it: then
-    `embedding_lookup` gives the same rows and the same gradient (summed in fp32, in token order, rounded once).  Anything
+    `embedding_lookup` gives the same rows and the same gradient (summed in fp32 in a fixed order, rounded once).  Anything
     else (frozen, wrapped by an adapter, hooked, norm-limited, sparse) stays the module's own."""
     if type(mod) is not torch.nn.Embedding or not torch.is_grad_enabled() or _has_any_global_hook():
         return False

@@ -1,8 +1,8 @@
 """`embedding_lookup`: scaled rows of a table, and the table's gradient by sorted tokens (csrc/embedding.cu).
 
 The reference's trunk calls the model's own embedding module (adapters/mlx_lm.py:140-164); the adapters here use this
-operator where the table is trained.  The gradient adds the rows of equal ids in the order of the tokens, in fp32,
-rounds once, and is the same bits for equal calls.
+operator where the table is trained.  The gradient adds the rows of equal ids in fp32 and in a fixed order, rounds
+once, and is the same bits for equal calls.
 """
 from __future__ import annotations
 

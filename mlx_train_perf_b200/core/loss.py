@@ -196,7 +196,8 @@ def device_status(device: torch.device) -> torch.Tensor:
 
 
 def check_device_status(device: torch.device | None = None) -> None:
-    """Synchronise and raise `DeviceTimeoutError` if any kernel reported a timed-out wait."""
+    """Synchronise and raise `DeviceTimeoutError` if any kernel reported a timed-out wait (`EmbeddingInputError` for an embedding id
+    outside its table)."""
     for idx, t in list(_status.items()):
         if device is not None and device.index is not None and idx != device.index:
             continue

@@ -1,9 +1,9 @@
 // Embedding lookup with scaling, and the gradient of its table by sorted tokens: what the adapters' trunk begins with
 // (adapters/mlx_lm.py:140-164 of the reference calls the model's own embedding module).
 //
-// Forward: y_i = scale W[id_i], a read and a write of N rows.  Backward: dW[v] = scale sum of dy_i over the i with id_i = v, in the order
-// of i, held in fp32 and rounded once; it reads N rows and writes all V rows, nearly all of them zero, so the writes bound
-// it.  No atomics, so equal calls give equal bits:
+// Forward: y_i = scale W[id_i], a read and a write of N rows.  Backward: dW[v] = scale sum of dy_i over the i with id_i = v, held in
+// fp32 and rounded once; it reads N rows and writes all V rows, nearly all of them zero, so the writes bound it.  The order
+// of a sum is fixed (token by token in a window, windows in turn) and there are no atomics, so equal calls give equal bits:
 //   1. one cluster sorts the tokens by id (stable, least digits first); beside it a second kernel fills the table with zeros, so that
 //      the sort's dependent steps cost nothing where the table is large (V = 151936, D = 4096: 170 us of writes at 7.3 TB/s);
 //   2. windows of the sorted tokens sum the rows of each run of equal ids; a run that lies in one window is written, one that

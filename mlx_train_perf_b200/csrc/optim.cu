@@ -181,7 +181,8 @@ __device__ __forceinline__ uint32_t mix(uint32_t pair, uint32_t step) {
   return x ^ (x >> 16);
 }
 
-// y > 0 to the e4m3 value below or above, up with a probability of the distance (dither uniform in [0, 2^20)); never zero.  Below 2^-6, where e4m3 values lie 2^-9 apart, 2^-6 is added first: sums in [2^-6, 2^-5) lie as far apart.
+// y > 0 to the e4m3 value below or above, up with a probability of the distance (dither uniform in [0, 2^20)); never zero.  Below 2^-6,
+// where e4m3 values lie 2^-9 apart, 2^-6 is added first: sums in [2^-6, 2^-5) lie as far apart.
 __device__ __forceinline__ float dithered(float y, uint32_t dither) {
   const float lift = y < 0x1p-6f ? 0x1p-6f : 0.f;
   const uint32_t u = __float_as_uint(y + lift) + dither;
