@@ -104,7 +104,7 @@ class _Call:
     """What one call hands the library, and what it got back.  The autograd functions below take it as their one argument beside
     `logps`: every further argument and output costs a training step host time (12 arguments and 3 outputs: 15 us of it)."""
     __slots__ = ("seqs", "mask", "cu", "old", "ref", "adv", "adv_strides", "rule", "from_nll", "per_sequence", "recorded", "out",
-                 "at", "shape", "dtype", "slopes")
+                 "at", "slopes_at", "shape", "dtype", "slopes")
 
     def args(self, logps) -> _lib.ObjectiveArgs:
         mask, cu, old, ref, adv = self.mask, self.cu, self.old, self.ref, self.adv
@@ -122,11 +122,11 @@ class _Call:
         with _lib.on(logps.device):                       # the blocks go by that device's SMs
             nbytes = lib.b200tp_objective_workspace_bytes(C.byref(a))
         self.at = nbytes // 4
-        count = self.seqs if self.per_sequence else 1
-        size = self.at + count + (logps.numel() if slopes else 0)
+        self.slopes_at = self.at + ((self.seqs if self.per_sequence else 1) + 3) // 4 * 4     # on a boundary of 16 bytes
+        size = self.slopes_at + (logps.numel() if slopes else 0)
         buf = torch.empty_strided((size,), (1,), dtype=torch.float32, device=logps.device)
-        weights = buf.data_ptr() + nbytes
-        return buf, nbytes, weights, weights + 4 * count if slopes else 0
+        base = buf.data_ptr()
+        return buf, nbytes, base + nbytes, base + 4 * self.slopes_at if slopes else 0
 
     def keep(self, ctx, logps, buf, slopes: bool):
         """Everything the gradient needs, apart from what the caller is given and may write to; the inputs are let go."""
@@ -147,8 +147,8 @@ class _Call:
                                cu is not None and cu.dtype is torch.int64, 0)
         if g.dtype is not torch.float32:
             g = g.to(torch.float32)
-        weights = buf.data_ptr() + 4 * self.at
-        slopes = weights + 4 * (self.seqs if self.per_sequence else 1) if self.slopes else None
+        base = buf.data_ptr()
+        weights, slopes = base + 4 * self.at, base + 4 * self.slopes_at if self.slopes else None
         with _lib.on(dev):
             rc = _lib.load().b200tp_objective_bwd(C.byref(a), slopes, weights, self.per_sequence, g.data_ptr(), at, _lib.stream(dev))
         _lib.check(rc)

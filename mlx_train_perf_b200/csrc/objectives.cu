@@ -26,6 +26,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kJoinThreads = 1024;
 constexpr int kUnroll = 4;
+constexpr int kShare = kThreads * 4;  // tokens of a block, on average
+constexpr int kFewTokens = kThreads * 2;
 
 struct Tokens {
   const void* cu;        // (S + 1) borders, or null: rows
@@ -53,6 +55,50 @@ __device__ __forceinline__ float ld(const float* p) { return *p; }
 __device__ __forceinline__ float ld(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void st(float* p, float v) { *p = v; }
 __device__ __forceinline__ void st(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// Four adjacent values, aligned to their size; four mask bytes.
+__device__ __forceinline__ void ld4(const float* p, float (&v)[4]) {
+  const float4 a = *reinterpret_cast<const float4*>(p);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+}
+__device__ __forceinline__ void ld4(const __nv_bfloat16* p, float (&v)[4]) {
+  const uint2 a = *reinterpret_cast<const uint2*>(p);
+  v[0] = __uint_as_float(a.x << 16);
+  v[1] = __uint_as_float(a.x & 0xffff0000u);
+  v[2] = __uint_as_float(a.y << 16);
+  v[3] = __uint_as_float(a.y & 0xffff0000u);
+}
+__device__ __forceinline__ void st4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void st4(__nv_bfloat16* p, const float (&v)[4]) {
+  uint2 a;
+  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&a);
+  h[0] = __floats2bfloat162_rn(v[0], v[1]);
+  h[1] = __floats2bfloat162_rn(v[2], v[3]);
+  *reinterpret_cast<uint2*>(p) = a;
+}
+__device__ __forceinline__ void ld4(const unsigned char* p, bool (&v)[4]) {
+  const uchar4 a = *reinterpret_cast<const uchar4*>(p);
+  v[0] = a.x != 0; v[1] = a.y != 0; v[2] = a.z != 0; v[3] = a.w != 0;
+}
+
+// Which tokens of [lo, hi) are taken four at a time: those of [i0, i1), where every array's token i0 lies on a boundary of four.  The
+// others, `rest` of them, one by one: single(v) for v in [0, rest).  Arrays that do not agree have no [i0, i1), and nor have shares of
+// so few tokens that four a thread would leave threads idle (8 x 61 tokens: 8.7 us in all by fours, 7.4 one by one).
+struct Fours {
+  int lo, i0, i1, rest;
+  __device__ __forceinline__ Fours(int lo_, int hi, int phase) : lo(lo_), i0(lo_), i1(lo_) {
+    if (phase >= 0 && hi - lo > kFewTokens) {
+      i0 = min(hi, lo + ((4 - ((phase + lo) & 3)) & 3));
+      i1 = i0 + (hi - i0) / 4 * 4;
+    }
+    rest = (i0 - lo) + (hi - i1);
+  }
+  __device__ __forceinline__ int single(int v) const { return v < i0 - lo ? lo + v : i1 + v - (i0 - lo); }
+};
+// Where a row's first token lies in its four, as one number for arrays that agree, else -1.
+template <typename T>
+__device__ __forceinline__ int phase_of(const T* row) { return static_cast<int>(reinterpret_cast<uintptr_t>(row) / sizeof(T)) & 3; }
+__device__ __forceinline__ int agree(int a, int b) { return a == b ? a : -1; }
 
 __device__ __forceinline__ long long border(const Tokens& t, long long s) {
   const long long b = t.cu_i64 ? static_cast<const long long*>(t.cu)[s] : static_cast<const int*>(t.cu)[s];
@@ -92,7 +138,7 @@ __device__ __forceinline__ void block_sums(double (&v)[K], double (*shared)[K]) 
 
 // exp(z) - 1 - z and exp(z) - 1 without cancellation: up to |z| = 1 the Taylor series to z^13 / 13!, whose first term left out
 // is 2 z^12 / 14! < 3e-11 of the sum; beyond, the library's expm1.  (Log ratios of a few tenths then leave hardly a warp with both
-// branches: 4 M tokens take 24 us, with the series up to 1/2 26.)
+// branches: a twelfth of the kernel's time against a series up to 1/2.)
 __device__ __forceinline__ float exp_minus_line(float z, float* minus_one) {
   if (fabsf(z) > 1.f) {
     *minus_one = expm1f(z);
@@ -141,7 +187,7 @@ policy_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ old, const
   }
   int lo, hi;
   share(t, s, k, lo, hi);
-  // rows, so that the loop indexes with 32 bits (126 instructions a token with 64)
+  // rows, so that the loop indexes with 32 bits (126 instructions a token with 64, 100 with 32, 76 four tokens at a time)
   const TX* x_row = x + s * t.x_stride;
   const TR* old_row = old + s * t.old_stride;
   const TR* ref_row = REF ? ref + s * t.ref_stride : nullptr;
@@ -152,50 +198,69 @@ policy_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ old, const
   const float adv_one = adv_each || lo >= hi ? 0.f : adv_row[0];
   double loss = 0., kl_sum = 0.;
   int count = 0, clips = 0;
-  for (int base = lo + threadIdx.x; base < hi; base += kThreads * kUnroll) {
-    float xv[kUnroll], ov[kUnroll], rv[kUnroll], av[kUnroll];
+  auto token = [&](bool on, float xv, float ov, float rv, float a) {          // the token's slope
+    if (!on) return 0.f;
+    const float u = t.sign * (xv - ov);
+    const bool up = a > 0.f && u > r.log_high, down = a < 0.f && u < r.log_low, clipped = up || down;
+    const float gain = a * (clipped ? (up ? r.high : r.low) : expf(u));
+    float slope = clipped ? 0.f : -gain;
+    float kl = 0.f;
+    if constexpr (REF) {
+      const float z = t.sign * (rv - xv);
+      float kl_slope;
+      if (r.kl_kind == B200TP_KL_K3) {
+        kl = exp_minus_line(z, &kl_slope);
+        kl_slope = -kl_slope;
+      } else if (r.kl_kind == B200TP_KL_K2) {
+        kl = 0.5f * z * z;
+        kl_slope = -z;
+      } else {
+        kl = -z;
+        kl_slope = 1.f;
+      }
+      if (r.kl_coef != 0.f) slope = fmaf(r.kl_coef, kl_slope, slope);
+      kl_sum += kl;
+    }
+    loss += r.kl_coef != 0.f ? fmaf(r.kl_coef, kl, -gain) : -gain;     // an infinite KL that is only reported stays out
+    count += 1;
+    clips += clipped;
+    return t.sign * slope;
+  };
+  int phase = agree(phase_of(x_row), phase_of(old_row));
+  if constexpr (REF) phase = agree(phase, phase_of(ref_row));
+  if (adv_each) phase = t.adv_tok == 1 ? agree(phase, phase_of(adv_row)) : -1;
+  if (mask_row != nullptr) phase = agree(phase, phase_of(mask_row));
+  if (slope_row != nullptr) phase = agree(phase, phase_of(slope_row));
+  const Fours f(lo, hi, phase);
+  for (int i = f.i0 + 4 * threadIdx.x; i < f.i1; i += 4 * kThreads) {
+    float xv[4], ov[4], rv[4] = {}, av[4] = {adv_one, adv_one, adv_one, adv_one}, sv[4];
+    bool on[4] = {true, true, true, true};
+    ld4(x_row + i, xv);
+    ld4(old_row + i, ov);
+    if constexpr (REF) ld4(ref_row + i, rv);
+    if (adv_each) ld4(adv_row + i, av);
+    if (mask_row != nullptr) ld4(mask_row + i, on);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sv[j] = token(on[j], xv[j], ov[j], rv[j], av[j]);
+    if (slope_row != nullptr) st4(slope_row + i, sv);
+  }
+  for (int base = threadIdx.x; base < f.rest; base += kThreads * kUnroll) {
+    float xv[kUnroll], ov[kUnroll], rv[kUnroll] = {}, av[kUnroll];
     bool on[kUnroll];
 #pragma unroll
-    for (int j = 0; j < kUnroll; ++j) {
-      const int i = base + j * kThreads, c = i < hi ? i : base;
-      on[j] = mask_row == nullptr || mask_row[c] != 0;
-      xv[j] = ld(x_row + c);
-      ov[j] = ld(old_row + c);
-      if constexpr (REF) rv[j] = ld(ref_row + c);
-      av[j] = adv_each ? adv_row[c * t.adv_tok] : adv_one;
+    for (int j = 0; j < kUnroll; ++j) {                               // all loads first
+      const int i = f.single(min(base + j * kThreads, f.rest - 1));
+      on[j] = mask_row == nullptr || mask_row[i] != 0;
+      xv[j] = ld(x_row + i);
+      ov[j] = ld(old_row + i);
+      if constexpr (REF) rv[j] = ld(ref_row + i);
+      av[j] = adv_each ? adv_row[i * t.adv_tok] : adv_one;
     }
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
-      const int i = base + j * kThreads;
-      if (i >= hi) break;
-      float slope = 0.f;
-      if (on[j]) {
-        const float u = t.sign * (xv[j] - ov[j]), a = av[j];
-        const bool up = a > 0.f && u > r.log_high, down = a < 0.f && u < r.log_low, clipped = up || down;
-        const float gain = a * (clipped ? (up ? r.high : r.low) : expf(u));
-        slope = clipped ? 0.f : -gain;
-        float kl = 0.f;
-        if constexpr (REF) {
-          const float z = t.sign * (rv[j] - xv[j]);
-          float kl_slope;
-          if (r.kl_kind == B200TP_KL_K3) {
-            kl = exp_minus_line(z, &kl_slope);
-            kl_slope = -kl_slope;
-          } else if (r.kl_kind == B200TP_KL_K2) {
-            kl = 0.5f * z * z;
-            kl_slope = -z;
-          } else {
-            kl = -z;
-            kl_slope = 1.f;
-          }
-          if (r.kl_coef != 0.f) slope = fmaf(r.kl_coef, kl_slope, slope);
-          kl_sum += kl;
-        }
-        loss += r.kl_coef != 0.f ? fmaf(r.kl_coef, kl, -gain) : -gain;     // an infinite KL that is only reported stays out
-        count += 1;
-        clips += clipped;
-      }
-      if (slope_row != nullptr) slope_row[i] = t.sign * slope;
+      if (base + j * kThreads >= f.rest) break;
+      const float slope = token(on[j], xv[j], ov[j], rv[j], av[j]);
+      if (slope_row != nullptr) slope_row[f.single(base + j * kThreads)] = slope;
     }
   }
   double all[4] = {loss, kl_sum, static_cast<double>(count), static_cast<double>(clips)};       // counts are exact
@@ -283,24 +348,37 @@ preference_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ ref, c
   const unsigned char* mask_row = t.mask == nullptr ? nullptr : t.mask + s * t.mask_stride;
   double sum = 0.;
   int count = 0;
-  for (int base = lo + threadIdx.x; base < hi; base += kThreads * kUnroll) {
-    float xv[kUnroll], rv[kUnroll];
+  auto token = [&](bool on, float xv, float rv) {
+    if (!on) return;
+    sum += REF ? static_cast<double>(xv) - rv : xv;
+    count += 1;
+  };
+  int phase = phase_of(x_row);
+  if constexpr (REF) phase = agree(phase, phase_of(ref_row));
+  if (mask_row != nullptr) phase = agree(phase, phase_of(mask_row));
+  const Fours f(lo, hi, phase);
+#pragma unroll 2
+  for (int i = f.i0 + 4 * threadIdx.x; i < f.i1; i += 4 * kThreads) {
+    float xv[4], rv[4] = {};
+    bool on[4] = {true, true, true, true};
+    ld4(x_row + i, xv);
+    if constexpr (REF) ld4(ref_row + i, rv);
+    if (mask_row != nullptr) ld4(mask_row + i, on);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) token(on[j], xv[j], rv[j]);
+  }
+  for (int base = threadIdx.x; base < f.rest; base += kThreads * kUnroll) {
+    float xv[kUnroll], rv[kUnroll] = {};
     bool on[kUnroll];
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
-      const int i = base + j * kThreads, c = i < hi ? i : base;
-      on[j] = i < hi && (mask_row == nullptr || mask_row[c] != 0);
-      xv[j] = ld(x_row + c);
-      if constexpr (REF) rv[j] = ld(ref_row + c);
+      const int i = f.single(min(base + j * kThreads, f.rest - 1));
+      on[j] = base + j * kThreads < f.rest && (mask_row == nullptr || mask_row[i] != 0);
+      xv[j] = ld(x_row + i);
+      if constexpr (REF) rv[j] = ld(ref_row + i);
     }
 #pragma unroll
-    for (int j = 0; j < kUnroll; ++j) {
-      if (!on[j]) continue;
-      double v = xv[j];
-      if constexpr (REF) v -= rv[j];
-      sum += v;
-      count += 1;
-    }
+    for (int j = 0; j < kUnroll; ++j) token(on[j], xv[j], rv[j]);
   }
   double all[2] = {sum * t.sign, static_cast<double>(count)};
   block_sums<kThreads>(all, sums);
@@ -377,29 +455,32 @@ objective_grad_kernel(const float* __restrict__ slopes, const float* __restrict_
   const float* slope_row = SLOPES ? slopes + s * out_stride : nullptr;
   TX* grad_row = grad + s * out_stride;
   const float w = *upstream * weights[per_seq ? s : 0];
-  for (int base = lo + threadIdx.x; base < hi; base += kThreads * kUnroll) {
-    float v[kUnroll];
-    bool on[kUnroll];
+  int phase = phase_of(grad_row);
+  if (mask_row != nullptr) phase = agree(phase, phase_of(mask_row));
+  if constexpr (SLOPES) phase = agree(phase, phase_of(slope_row));
+  const Fours f(lo, hi, phase);
+#pragma unroll 2
+  for (int i = f.i0 + 4 * threadIdx.x; i < f.i1; i += 4 * kThreads) {
+    float v[4] = {1.f, 1.f, 1.f, 1.f};
+    bool on[4] = {true, true, true, true};
+    if constexpr (SLOPES) ld4(slope_row + i, v);
+    if (mask_row != nullptr) ld4(mask_row + i, on);
 #pragma unroll
-    for (int j = 0; j < kUnroll; ++j) {
-      const int i = base + j * kThreads, c = i < hi ? i : base;
-      on[j] = mask_row == nullptr || mask_row[c] != 0;
-      v[j] = SLOPES ? slope_row[c] : 1.f;
-    }
-#pragma unroll
-    for (int j = 0; j < kUnroll; ++j) {
-      const int i = base + j * kThreads;
-      if (i < hi) st(grad_row + i, on[j] ? w * v[j] : 0.f);
-    }
+    for (int j = 0; j < 4; ++j) v[j] = on[j] ? w * v[j] : 0.f;
+    st4(grad_row + i, v);
+  }
+#pragma unroll 4
+  for (int v = threadIdx.x; v < f.rest; v += kThreads) {
+    const int i = f.single(v);
+    st(grad_row + i, mask_row == nullptr || mask_row[i] != 0 ? w * (SLOPES ? slope_row[i] : 1.f) : 0.f);
   }
 }
 
-// Blocks a sequence: about 1024 tokens each on average (one round of loads a thread), at most eight blocks an SM in all and at most
-// 512 a sequence.
+// Blocks a sequence: about 1024 tokens each on average, at most eight blocks an SM in all and at most 512 a sequence.
 int splits_of(long long seqs, long long length, bool packed) {
   const int64_t mean = packed ? ceil_div(length, seqs) : length;
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(512, 8ll * sm_count() / seqs));
-  return static_cast<int>(std::max<int64_t>(1, std::min(most, ceil_div(mean, kThreads * kUnroll))));
+  return static_cast<int>(std::max<int64_t>(1, std::min(most, ceil_div(mean, kShare))));
 }
 
 int check(const b200tp_objective_args* a) {

@@ -87,7 +87,7 @@ def _close(got, ref, tol, store=E32):
     assert not torch.isnan(got).any() and worst <= 0.0, worst
 
 
-CASES = [(2, 1, False), (2, 1, True), (4, 33, False), (6, 257, True), (8, 5000, False), (2, 70001, True), (3000, 3, False), (10, 0, False)]
+CASES = [(2, 1, False), (2, 1, True), (4, 33, False), (6, 257, True), (8, 5000, False), (2, 70001, True), (4, 2051, False), (3000, 3, False), (10, 0, False)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -286,6 +286,29 @@ def test_strided_rows_and_empty_masks(cuda_device):
     preference_loss(row.expand(6, -1), r.to(dev)).loss.backward()
     preference_loss(full, r.to(dev)).loss.backward()
     torch.testing.assert_close(row.grad, full.grad.sum(0), rtol=0, atol=6 * E32 * full.grad.abs().sum(0).max().item())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("offsets", [(0, 0, 0, 0), (1, 1, 1, 1), (3, 3, 3, 3), (0, 1, 0, 0), (2, 0, 0, 0), (0, 0, 0, 3), (0, 0, 2, 0)])
+def test_arrays_that_begin_anywhere(cuda_device, offsets, dtype):
+    """Rows of 3001 tokens whose arrays begin on and off a boundary of four tokens, alike and not: the gradients of contiguous copies,
+    bit for bit, and their sums up to the order of additions in double."""
+    dev = cuda_device
+    g = torch.Generator().manual_seed(27)
+    wide = lambda t, o: torch.cat([torch.zeros(4, o, dtype=t.dtype), t, torch.zeros(4, 8 - o, dtype=t.dtype)], 1).to(dev)[:, o:o + 3001]
+    x, o, r, mask, _, _ = _tokens(4, 3001, False, dtype, 29)
+    a = torch.randn(x.shape, generator=g)
+    got = []
+    for place in (lambda t, k: t.to(dev), lambda t, k: wide(t, offsets[k])):
+        leaf = place(x, 0).detach().requires_grad_(True)
+        ol, rl, ml, al = place(o, 1), place(r, 2), place(mask, 3), place(a, 2)
+        p = policy_loss(leaf, ol, al, ref_logps=rl, mask=ml, kl_coef=0.2)
+        q = preference_loss(leaf, rl, mask=ml, beta=0.01)
+        got.append((p.loss, p.kl, q.loss, torch.autograd.grad(p.loss, leaf)[0], torch.autograd.grad(q.loss, leaf)[0]))
+    for u, v in zip(got[0][:3], got[1][:3]):
+        assert abs(u.item() - v.item()) <= 2 * E32 * abs(v.item()) + 1e-12
+    assert torch.equal(got[0][3], got[1][3])
+    assert (got[0][4] - got[1][4]).abs().max() <= 2 * STORE[dtype] * got[1][4].abs().max()   # its weight follows the sums
 
 
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
