@@ -40,7 +40,7 @@ template <int BITS>
 constexpr int kChunk = BITS == 8 ? kRound : 2 * kRound;
 constexpr int kTensors = 600;               // of one launch: 26 kB of its parameters
 constexpr int kNear = 64;                   // entries of the coarse index
-constexpr int kFew = 48;                    // of the small form: 2 kB
+constexpr int kFew = 48;                    // of the small form: 2 kB, 5.9 us of host time for 48 tensors against 11.3 (one: 4.5, 6.3)
 
 struct Rule {
   float beta1, beta2, one_beta1, one_beta2;

@@ -86,6 +86,21 @@ def test_gradient_is_exact_where_the_sums_are(cuda_device):
         assert torch.equal(grad.double(), _gradient_ref(ids, dy, v, 2.0)[0])
 
 
+def test_gradient_against_differences(cuda_device):
+    """The lookup is linear in its table: along any direction V, sum(dy * (f(W + V) - f(W))) is sum(dW * V), exactly where all values are
+    whole numbers."""
+    dev = cuda_device
+    g = torch.Generator().manual_seed(6)
+    whole = lambda *s: torch.randint(-6, 7, s, generator=g).float().to(dev)
+    for n, v, d in ((50, 20, 24), (3000, 400, 72)):
+        ids = _ids(n, v, "words", g).to(dev)
+        w, way, dy = whole(v, d).requires_grad_(True), whole(v, d), whole(n, d)
+        out = embedding_lookup(ids, w, scale=3.0)
+        grad, = torch.autograd.grad(out, w, dy)
+        moved = embedding_lookup(ids, w.detach() + way, scale=3.0)
+        assert (dy.double() * (moved - out.detach()).double()).sum() == (grad.double() * way.double()).sum()
+
+
 def test_order_of_the_sum_is_the_tokens_own(cuda_device):
     """Large and small values of one id: fp32 sums depend on the order, and the order is that of the tokens within a window (8 rows here,
     one id, one window)."""
