@@ -6,16 +6,18 @@
 // [cu[s], cu[s + 1]).  A token that its mask leaves out takes no part whatever it holds: values are selected, never
 // multiplied by zero.
 //
-// Both losses are one pass over the tokens, then one block that joins the sequences' sums, then (backward) one pass that
-// writes the gradient.  A token costs 9 to 21 bytes and a few dozen operations, so long batches are bound by HBM and the
+// Both losses are one pass over the tokens, then one block that joins the sequences' sums (up to eight blocks are one cluster, whose
+// first block joins: no second launch), then (backward) one pass that writes the gradient.  A token costs 9 to 21 bytes and a few dozen operations, so long batches are bound by HBM and the
 // usual ones by launches: the pass and the join are two launches, the second one programmatic, and nothing is zeroed
 // beforehand (no counter, no atomics: sums are formed in a fixed order, in double, since what is left after
 // advantages of both signs cancel is small beside the terms).
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 #include "ptx.cuh"
@@ -23,8 +25,11 @@
 namespace b200tp {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kThreads = 256;
 constexpr int kJoinThreads = 1024;
+constexpr unsigned kClusterMost = 8;
 constexpr int kUnroll = 4;
 constexpr int kShare = kThreads * 4;  // tokens of a block, on average
 constexpr int kFewTokens = kThreads * 2;
@@ -161,28 +166,163 @@ __device__ __forceinline__ float exp_minus_line(float z, float* minus_one) {
   return s;
 }
 
+// A sequence's parts joined.  Up to eight: each thread of the warp does its own sequence `s`.  More: the warp's lanes share one.
+__device__ __forceinline__ Part joined(const Part* parts, const Tokens& t, long long s) {
+  Part p{0., 0., 0., 0.};
+  for (int k = 0; k < t.splits; ++k) {
+    const Part q = parts[s * t.splits + k];
+    p.loss += q.loss;
+    p.kl += q.kl;
+    p.count += q.count;
+    p.clipped += q.clipped;
+  }
+  return p;
+}
+__device__ __forceinline__ Part joined_by_warp(const Part* parts, const Tokens& t, long long s) {
+  double v[4] = {0., 0., 0., 0.};
+#pragma unroll 4
+  for (int k = threadIdx.x & 31; k < t.splits; k += 32) {
+    const Part q = parts[s * t.splits + k];
+    v[0] += q.loss;
+    v[1] += q.kl;
+    v[2] += q.count;
+    v[3] += q.clipped;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  return Part{v[0], v[1], v[2], v[3]};
+}
+constexpr int kFewParts = 8;
+
+// One block of N threads: the sequences' sums, then the batch's.
+struct PolicyJoin {
+  int normalize;
+  float *weights, *loss, *stats;
+};
+template <int N>
+__device__ __forceinline__ void join(const Part* parts, const Tokens& t, const PolicyJoin& o) {
+  const int normalize = o.normalize;
+  float *weights = o.weights, *loss_out = o.loss, *stats = o.stats;
+  __shared__ double sums[N / 32][4];
+  double all[4] = {0., 0., 0., 0.};           // loss, kl, taken and clipped tokens
+  const bool few = t.splits <= kFewParts;
+  const int step = few ? N : N / 32;
+  for (long long s = few ? threadIdx.x : threadIdx.x >> 5; s < t.seqs; s += step) {
+    const Part p = few ? joined(parts, t, s) : joined_by_warp(parts, t, s);
+    if (!few && (threadIdx.x & 31) != 0) continue;
+    double l = p.loss;
+    if (normalize == B200TP_NORMALIZE_SEQUENCE) {
+      const double w = 1. / (static_cast<double>(t.seqs) * max(p.count, 1.));
+      l *= w;
+      weights[s] = static_cast<float>(w);
+    }
+    all[0] += l;
+    all[1] += p.kl;
+    all[2] += p.count;
+    all[3] += p.clipped;
+  }
+  block_sums<N>(all, sums);
+  const double loss = all[0], kl = all[1], count = all[2], clipped = all[3];
+  if (threadIdx.x == 0) {
+    const double per = 1. / max(count, 1.);
+    if (normalize != B200TP_NORMALIZE_SEQUENCE) weights[0] = normalize == B200TP_NORMALIZE_TOKEN ? static_cast<float>(per) : 1.f;
+    *loss_out = static_cast<float>(normalize == B200TP_NORMALIZE_TOKEN ? loss * per : loss);
+    stats[0] = static_cast<float>(kl * per);
+    stats[1] = static_cast<float>(clipped * per);
+  }
+}
+
+// One block of N threads: pair i is the sequences i and P + i.  h = beta (l_i - l_{P + i}) - margin; out: the loss, the S rewards
+// beta l_s, and for each sequence the weight that the loss's gradient gives every taken token of it.
+struct PreferenceJoin {
+  int kind;
+  double beta, smoothing, margin;
+  int average;
+  float *loss, *rewards, *weights;
+};
+template <int N>
+__device__ __forceinline__ void join(const Part* parts, const Tokens& t, const PreferenceJoin& o) {
+  const int kind = o.kind, average = o.average;
+  const double beta = o.beta, smoothing = o.smoothing, margin = o.margin;
+  float *loss_out = o.loss, *rewards = o.rewards, *weights = o.weights;
+  __shared__ double sums[N / 32][1];
+  const long long pairs = t.seqs / 2;
+  double total = 0.;
+  const bool few = t.splits <= kFewParts;
+  const int step = few ? N : N / 32;
+  for (long long i = few ? threadIdx.x : threadIdx.x >> 5; i < pairs; i += step) {
+    const Part c = few ? joined(parts, t, i) : joined_by_warp(parts, t, i);
+    const Part r = few ? joined(parts, t, pairs + i) : joined_by_warp(parts, t, pairs + i);
+    if (!few && (threadIdx.x & 31) != 0) continue;
+    const double cs = average ? 1. / max(c.count, 1.) : 1., rs = average ? 1. / max(r.count, 1.) : 1.;
+    const double lc = c.loss * cs, lr = r.loss * rs;
+    const double h = beta * (lc - lr) - margin;
+    double f, slope;
+    if (kind == B200TP_PREFERENCE_SIGMOID) {
+      const double e = exp(-fabs(h)), tail = log1p(e);
+      f = (1. - smoothing) * (tail + max(-h, 0.));
+      if (smoothing > 0.) f += smoothing * (tail + max(h, 0.));       // an infinite h must not meet a factor of zero
+      slope = smoothing - (h >= 0. ? e : 1.) / (1. + e);             // smoothing - sigmoid(-h)
+    } else if (kind == B200TP_PREFERENCE_HINGE) {
+      f = h > 1. ? 0. : 1. - h;
+      slope = h < 1. ? -1. : 0.;
+    } else {
+      const double off = (h - 0.5) / beta;
+      f = off * off;
+      slope = 2. * off / beta;
+    }
+    if (isnan(h)) f = slope = h;                                      // comparisons above would hide it
+    total += f;
+    const double w = t.sign * beta * slope / static_cast<double>(pairs);
+    weights[i] = static_cast<float>(w * cs);
+    weights[pairs + i] = static_cast<float>(-w * rs);
+    rewards[i] = static_cast<float>(beta * lc);
+    rewards[pairs + i] = static_cast<float>(beta * lr);
+  }
+  double all[1] = {total};
+  block_sums<N>(all, sums);
+  if (threadIdx.x == 0) *loss_out = static_cast<float>(all[0] / static_cast<double>(pairs));
+}
+
+template <typename Join>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Part* parts, const Tokens t, const Join o) {
+  griddep_wait();
+  griddep_launch_dependents();
+  join<kJoinThreads>(parts, t, o);
+}
+
+// The last step of a block of tokens that is one of a cluster: the first of them joins all parts.
+template <typename Join>
+__device__ __forceinline__ void join_in_cluster(const Part* parts, const Tokens& t, const Join& o) {
+  cg::this_cluster().sync();                      // the parts of all blocks are written, and seen by all
+  if (blockIdx.x == 0) join<kThreads>(parts, t, o);
+}
+
 // Per token:  u = x - o, ratio = exp(u);  clipped iff A > 0 and u > log(1 + high), or A < 0 and u < log(1 - low), which is
 // where min(ratio A, clip(ratio) A) takes the constant (decided on u, an exact difference for near values, and not
 // on the rounded exponential);  f = -A (clipped ? bound : ratio) + c kl;  slope = (clipped ? 0 : -A ratio) + c kl'.
 // Slopes are kept without their weight (1 / count is known only after all tokens): 4 bytes written here and read
 // again by the backward, where computing them anew would read 13 or more.
-template <typename TX, typename TR, bool REF>
+template <typename TX, typename TR, bool REF, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads)
 policy_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ old, const TR* __restrict__ ref,
                      const float* __restrict__ adv, const Tokens t, const PolicyRule r, float* __restrict__ slopes,
-                     Part* __restrict__ parts) {
+                     Part* __restrict__ parts, const PolicyJoin o) {
   griddep_wait();
   griddep_launch_dependents();
   __shared__ double sums[kThreads / 32][4];
   const long long s = blockIdx.x / t.splits;
   const int k = static_cast<int>(blockIdx.x % t.splits);
   const long long out_stride = t.cu != nullptr ? 0 : t.length;
-  if (s == t.seqs) {                 // packed tokens outside every sequence: no slope
-    if (slopes != nullptr && k == 0 && t.cu != nullptr) {
+  if (s >= t.seqs) {                 // packed tokens outside every sequence: no slope
+    if (slopes != nullptr && s == t.seqs && k == 0 && t.cu != nullptr) {
       const long long first = border(t, 0), last = border(t, t.seqs);
       for (long long i = threadIdx.x; i < first; i += kThreads) slopes[i] = 0.f;
       for (long long i = max(first, last) + threadIdx.x; i < t.length; i += kThreads) slopes[i] = 0.f;
     }
+    if constexpr (CLUSTER) join_in_cluster(parts, t, o);
     return;
   }
   int lo, hi;
@@ -266,81 +406,24 @@ policy_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ old, const
   double all[4] = {loss, kl_sum, static_cast<double>(count), static_cast<double>(clips)};       // counts are exact
   block_sums<kThreads>(all, sums);
   if (threadIdx.x == 0) parts[blockIdx.x] = Part{all[0], all[1], all[2], all[3]};
-}
-
-// A sequence's parts joined.  Up to eight: each thread of the warp does its own sequence `s`.  More: the warp's lanes share one.
-__device__ __forceinline__ Part joined(const Part* parts, const Tokens& t, long long s) {
-  Part p{0., 0., 0., 0.};
-  for (int k = 0; k < t.splits; ++k) {
-    const Part q = parts[s * t.splits + k];
-    p.loss += q.loss;
-    p.kl += q.kl;
-    p.count += q.count;
-    p.clipped += q.clipped;
-  }
-  return p;
-}
-__device__ __forceinline__ Part joined_by_warp(const Part* parts, const Tokens& t, long long s) {
-  double v[4] = {0., 0., 0., 0.};
-#pragma unroll 4
-  for (int k = threadIdx.x & 31; k < t.splits; k += 32) {
-    const Part q = parts[s * t.splits + k];
-    v[0] += q.loss;
-    v[1] += q.kl;
-    v[2] += q.count;
-    v[3] += q.clipped;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-  return Part{v[0], v[1], v[2], v[3]};
-}
-constexpr int kFewParts = 8;
-
-// One block: the sequences' sums, then the batch's.
-__global__ void __launch_bounds__(kJoinThreads)
-policy_join_kernel(const Part* __restrict__ parts, const Tokens t, int normalize, float* __restrict__ weights,
-                   float* __restrict__ loss_out, float* __restrict__ stats) {
-  griddep_wait();
-  griddep_launch_dependents();
-  __shared__ double sums[kJoinThreads / 32][4];
-  double all[4] = {0., 0., 0., 0.};           // loss, kl, taken and clipped tokens
-  const bool few = t.splits <= kFewParts;
-  const int step = few ? kJoinThreads : kJoinThreads / 32;
-  for (long long s = few ? threadIdx.x : threadIdx.x >> 5; s < t.seqs; s += step) {
-    const Part p = few ? joined(parts, t, s) : joined_by_warp(parts, t, s);
-    if (!few && (threadIdx.x & 31) != 0) continue;
-    double l = p.loss;
-    if (normalize == B200TP_NORMALIZE_SEQUENCE) {
-      const double w = 1. / (static_cast<double>(t.seqs) * max(p.count, 1.));
-      l *= w;
-      weights[s] = static_cast<float>(w);
-    }
-    all[0] += l;
-    all[1] += p.kl;
-    all[2] += p.count;
-    all[3] += p.clipped;
-  }
-  block_sums<kJoinThreads>(all, sums);
-  const double loss = all[0], kl = all[1], count = all[2], clipped = all[3];
-  if (threadIdx.x == 0) {
-    const double per = 1. / max(count, 1.);
-    if (normalize != B200TP_NORMALIZE_SEQUENCE) weights[0] = normalize == B200TP_NORMALIZE_TOKEN ? static_cast<float>(per) : 1.f;
-    *loss_out = static_cast<float>(normalize == B200TP_NORMALIZE_TOKEN ? loss * per : loss);
-    stats[0] = static_cast<float>(kl * per);
-    stats[1] = static_cast<float>(clipped * per);
-  }
+  if constexpr (CLUSTER) join_in_cluster(parts, t, o);
 }
 
 // Sum of the masked log ratios x - r of a sequence's share.
-template <typename TX, typename TR, bool REF>
+template <typename TX, typename TR, bool REF, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads)
-preference_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ ref, const Tokens t, Part* __restrict__ parts) {
+preference_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ ref, const Tokens t, Part* __restrict__ parts,
+                         const PreferenceJoin o) {
   griddep_wait();
   griddep_launch_dependents();
   __shared__ double sums[kThreads / 32][2];
   const long long s = blockIdx.x / t.splits;
+  if constexpr (CLUSTER) {
+    if (s >= t.seqs) {                // fills up the cluster
+      join_in_cluster(parts, t, o);
+      return;
+    }
+  }
   int lo, hi;
   share(t, s, static_cast<int>(blockIdx.x % t.splits), lo, hi);
   const TX* x_row = x + s * t.x_stride;
@@ -383,52 +466,7 @@ preference_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ ref, c
   double all[2] = {sum * t.sign, static_cast<double>(count)};
   block_sums<kThreads>(all, sums);
   if (threadIdx.x == 0) parts[blockIdx.x] = Part{all[0], 0., all[1], 0.};
-}
-
-// One block: pair i is the sequences i and P + i.  h = beta (l_i - l_{P + i}) - margin; out: the loss, the S rewards
-// beta l_s, and for each sequence the weight that the loss's gradient gives every taken token of it.
-__global__ void __launch_bounds__(kJoinThreads)
-preference_join_kernel(const Part* __restrict__ parts, const Tokens t, int kind, double beta, double smoothing, double margin,
-                       int average, float* __restrict__ loss_out, float* __restrict__ rewards, float* __restrict__ weights) {
-  griddep_wait();
-  griddep_launch_dependents();
-  __shared__ double sums[kJoinThreads / 32][1];
-  const long long pairs = t.seqs / 2;
-  double total = 0.;
-  const bool few = t.splits <= kFewParts;
-  const int step = few ? kJoinThreads : kJoinThreads / 32;
-  for (long long i = few ? threadIdx.x : threadIdx.x >> 5; i < pairs; i += step) {
-    const Part c = few ? joined(parts, t, i) : joined_by_warp(parts, t, i);
-    const Part r = few ? joined(parts, t, pairs + i) : joined_by_warp(parts, t, pairs + i);
-    if (!few && (threadIdx.x & 31) != 0) continue;
-    const double cs = average ? 1. / max(c.count, 1.) : 1., rs = average ? 1. / max(r.count, 1.) : 1.;
-    const double lc = c.loss * cs, lr = r.loss * rs;
-    const double h = beta * (lc - lr) - margin;
-    double f, slope;
-    if (kind == B200TP_PREFERENCE_SIGMOID) {
-      const double e = exp(-fabs(h)), tail = log1p(e);
-      f = (1. - smoothing) * (tail + max(-h, 0.));
-      if (smoothing > 0.) f += smoothing * (tail + max(h, 0.));       // an infinite h must not meet a factor of zero
-      slope = smoothing - (h >= 0. ? e : 1.) / (1. + e);             // smoothing - sigmoid(-h)
-    } else if (kind == B200TP_PREFERENCE_HINGE) {
-      f = h > 1. ? 0. : 1. - h;
-      slope = h < 1. ? -1. : 0.;
-    } else {
-      const double off = (h - 0.5) / beta;
-      f = off * off;
-      slope = 2. * off / beta;
-    }
-    if (isnan(h)) f = slope = h;                                      // comparisons above would hide it
-    total += f;
-    const double w = t.sign * beta * slope / static_cast<double>(pairs);
-    weights[i] = static_cast<float>(w * cs);
-    weights[pairs + i] = static_cast<float>(-w * rs);
-    rewards[i] = static_cast<float>(beta * lc);
-    rewards[pairs + i] = static_cast<float>(beta * lr);
-  }
-  double all[1] = {total};
-  block_sums<kJoinThreads>(all, sums);
-  if (threadIdx.x == 0) *loss_out = static_cast<float>(all[0] / static_cast<double>(pairs));
+  if constexpr (CLUSTER) join_in_cluster(parts, t, o);
 }
 
 // grad = upstream * weight * (slopes ? slope : mask).  `per_seq`: a weight for each sequence, else one.
@@ -523,26 +561,64 @@ int check_workspace(const b200tp_objective_args* a, void* workspace, size_t byte
   return B200TP_OK;
 }
 
-template <typename TX, typename TR>
-int launch_policy(const b200tp_objective_args* a, const Tokens& t, const PolicyRule& r, float* slopes, Part* parts,
-                  cudaStream_t stream) {
-  auto go = [&](auto kernel) {
-    return launch_pdl(kernel, dim3(blocks_of(t, slopes != nullptr)), dim3(kThreads), 0, stream, static_cast<const TX*>(a->logps),
-                      static_cast<const TR*>(a->old_logps), static_cast<const TR*>(a->ref_logps),
-                      static_cast<const float*>(a->advantages), t, r, slopes, parts);
-  };
-  B200TP_CUDA_OK(a->ref_logps != nullptr ? go(policy_tokens_kernel<TX, TR, true>) : go(policy_tokens_kernel<TX, TR, false>));
+// A tokens kernel and its join: one launch of a cluster of 2, 4 or 8 blocks where that holds them all (8 x 61 tokens, forward and backward: 6.5 us on the
+// device against 7.8, and 2 us less of host time), else two launches.
+template <typename Join, typename Go>
+int launch_both(unsigned blocks, const Part* parts, const Tokens& t, const Join& o, cudaStream_t stream, Go go) {
+  if (blocks <= kClusterMost) {
+    unsigned size = 1;
+    while (size < blocks) size *= 2;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    B200TP_CUDA_OK(go(cfg, std::true_type{}));
+    return B200TP_OK;
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  B200TP_CUDA_OK(go(cfg, std::false_type{}));
+  B200TP_CUDA_OK(launch_pdl(join_kernel<Join>, dim3(1), dim3(kJoinThreads), 0, stream, parts, t, o));
   return B200TP_OK;
 }
 
 template <typename TX, typename TR>
-int launch_preference(const b200tp_objective_args* a, const Tokens& t, Part* parts, cudaStream_t stream) {
-  auto go = [&](auto kernel) {
-    return launch_pdl(kernel, dim3(blocks_of(t, false)), dim3(kThreads), 0, stream, static_cast<const TX*>(a->logps),
-                      static_cast<const TR*>(a->ref_logps), t, parts);
-  };
-  B200TP_CUDA_OK(a->ref_logps != nullptr ? go(preference_tokens_kernel<TX, TR, true>) : go(preference_tokens_kernel<TX, TR, false>));
-  return B200TP_OK;
+int launch_policy(const b200tp_objective_args* a, const Tokens& t, const PolicyRule& r, float* slopes, Part* parts,
+                  const PolicyJoin& o, cudaStream_t stream) {
+  const TX* x = static_cast<const TX*>(a->logps);
+  const TR *old = static_cast<const TR*>(a->old_logps), *ref = static_cast<const TR*>(a->ref_logps);
+  const float* adv = static_cast<const float*>(a->advantages);
+  return launch_both(blocks_of(t, slopes != nullptr), parts, t, o, stream, [&](const cudaLaunchConfig_t& cfg, auto cluster) {
+    constexpr bool kIn = decltype(cluster)::value;
+    return ref != nullptr ? cudaLaunchKernelEx(&cfg, policy_tokens_kernel<TX, TR, true, kIn>, x, old, ref, adv, t, r, slopes, parts, o)
+                          : cudaLaunchKernelEx(&cfg, policy_tokens_kernel<TX, TR, false, kIn>, x, old, ref, adv, t, r, slopes, parts, o);
+  });
+}
+
+template <typename TX, typename TR>
+int launch_preference(const b200tp_objective_args* a, const Tokens& t, Part* parts, const PreferenceJoin& o, cudaStream_t stream) {
+  const TX* x = static_cast<const TX*>(a->logps);
+  const TR* ref = static_cast<const TR*>(a->ref_logps);
+  return launch_both(blocks_of(t, false), parts, t, o, stream, [&](const cudaLaunchConfig_t& cfg, auto cluster) {
+    constexpr bool kIn = decltype(cluster)::value;
+    return ref != nullptr ? cudaLaunchKernelEx(&cfg, preference_tokens_kernel<TX, TR, true, kIn>, x, ref, t, parts, o)
+                          : cudaLaunchKernelEx(&cfg, preference_tokens_kernel<TX, TR, false, kIn>, x, ref, t, parts, o);
+  });
 }
 
 }  // namespace
@@ -574,16 +650,12 @@ int b200tp_preference_loss_fwd(const b200tp_objective_args* a, int32_t kind, dou
   const Tokens t = tokens(a);
   Part* parts = static_cast<Part*>(workspace);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  const PreferenceJoin o{kind, beta, label_smoothing, margin, average, loss, rewards, weights};
   if (a->dtype == B200TP_BF16)
-    rc = a->other_dtype == B200TP_BF16 ? launch_preference<__nv_bfloat16, __nv_bfloat16>(a, t, parts, stream)
-                                       : launch_preference<__nv_bfloat16, float>(a, t, parts, stream);
-  else
-    rc = a->other_dtype == B200TP_BF16 ? launch_preference<float, __nv_bfloat16>(a, t, parts, stream)
-                                       : launch_preference<float, float>(a, t, parts, stream);
-  if (rc) return rc;
-  B200TP_CUDA_OK(launch_pdl(preference_join_kernel, dim3(1), dim3(kJoinThreads), 0, stream, static_cast<const Part*>(parts), t, kind,
-                            beta, label_smoothing, margin, average, loss, rewards, weights));
-  return B200TP_OK;
+    return a->other_dtype == B200TP_BF16 ? launch_preference<__nv_bfloat16, __nv_bfloat16>(a, t, parts, o, stream)
+                                         : launch_preference<__nv_bfloat16, float>(a, t, parts, o, stream);
+  return a->other_dtype == B200TP_BF16 ? launch_preference<float, __nv_bfloat16>(a, t, parts, o, stream)
+                                       : launch_preference<float, float>(a, t, parts, o, stream);
 }
 
 int b200tp_policy_loss_fwd(const b200tp_objective_args* a, double clip_low, double clip_high, double kl_coef, int32_t kl_kind,
@@ -614,16 +686,12 @@ int b200tp_policy_loss_fwd(const b200tp_objective_args* a, double clip_low, doub
   r.kl_kind = kl_kind;
   Part* parts = static_cast<Part*>(workspace);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  const PolicyJoin o{normalize, weights, loss, stats};
   if (a->dtype == B200TP_BF16)
-    rc = a->other_dtype == B200TP_BF16 ? launch_policy<__nv_bfloat16, __nv_bfloat16>(a, t, r, slopes, parts, stream)
-                                       : launch_policy<__nv_bfloat16, float>(a, t, r, slopes, parts, stream);
-  else
-    rc = a->other_dtype == B200TP_BF16 ? launch_policy<float, __nv_bfloat16>(a, t, r, slopes, parts, stream)
-                                       : launch_policy<float, float>(a, t, r, slopes, parts, stream);
-  if (rc) return rc;
-  B200TP_CUDA_OK(launch_pdl(policy_join_kernel, dim3(1), dim3(kJoinThreads), 0, stream, static_cast<const Part*>(parts), t, normalize,
-                            weights, loss, stats));
-  return B200TP_OK;
+    return a->other_dtype == B200TP_BF16 ? launch_policy<__nv_bfloat16, __nv_bfloat16>(a, t, r, slopes, parts, o, stream)
+                                         : launch_policy<__nv_bfloat16, float>(a, t, r, slopes, parts, o, stream);
+  return a->other_dtype == B200TP_BF16 ? launch_policy<float, __nv_bfloat16>(a, t, r, slopes, parts, o, stream)
+                                       : launch_policy<float, float>(a, t, r, slopes, parts, o, stream);
 }
 
 int b200tp_objective_bwd(const b200tp_objective_args* a, const float* slopes, const float* weights, int32_t per_sequence,
