@@ -22,6 +22,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.h"
 #include "ptx.cuh"
@@ -519,13 +520,27 @@ int launch_direct(const b200tp_embedding_args* a, const void* dy, void* dw, cuda
   return B200TP_OK;
 }
 
+constexpr size_t sort_smem(int digit) { return static_cast<size_t>(kSortWarps + 2) * (size_t{4} << digit); }
+
+// The most shared memory a sort may ask for, once for each device.
+int configure_sort() {
+  static std::atomic<int> configured[64];
+  int dev = 0;
+  B200TP_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= 0 && dev < 64 && configured[dev].load(std::memory_order_acquire)) return B200TP_OK;
+  const int most = static_cast<int>(sort_smem(kMaxDigit));
+  B200TP_CUDA_OK(cudaFuncSetAttribute(embed_sort_kernel<int>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+  B200TP_CUDA_OK(cudaFuncSetAttribute(embed_sort_kernel<long long>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+  if (dev >= 0 && dev < 64) configured[dev].store(1, std::memory_order_release);
+  return B200TP_OK;
+}
+
 template <typename ID>
 int launch_sort(const b200tp_embedding_args* a, const Sort& s, void* dw, cudaStream_t stream, int* status) {
   const long long bytes = a->v * a->d * (a->dtype == B200TP_BF16 ? 2 : 4);
-  const size_t smem = static_cast<size_t>(kSortWarps + 2) * (size_t{4} << s.digit);
-  if (smem > 48 << 10)
-    B200TP_CUDA_OK(cudaFuncSetAttribute(embed_sort_kernel<ID>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  B200TP_CUDA_OK(launch_pdl(embed_sort_kernel<ID>, dim3(kCluster), dim3(kSortThreads), smem, stream, static_cast<const ID*>(a->ids), s,
+  const int rc = configure_sort();
+  if (rc) return rc;
+  B200TP_CUDA_OK(launch_pdl(embed_sort_kernel<ID>, dim3(kCluster), dim3(kSortThreads), sort_smem(s.digit), stream, static_cast<const ID*>(a->ids), s,
                             status));
   B200TP_CUDA_OK(launch_pdl(embed_fill_kernel, dim3(static_cast<unsigned>(ceil_div(bytes, kFillBytes))), dim3(kSortThreads), 0, stream,
                             static_cast<uint4*>(dw), static_cast<long long>(bytes)));

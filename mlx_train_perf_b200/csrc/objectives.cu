@@ -7,10 +7,10 @@
 // multiplied by zero.
 //
 // Both losses are one pass over the tokens, then one block that joins the sequences' sums (up to eight blocks are one cluster, whose
-// first block joins: no second launch), then (backward) one pass that writes the gradient.  A token costs 9 to 21 bytes and a few dozen operations, so long batches are bound by HBM and the
-// usual ones by launches: the pass and the join are two launches, the second one programmatic, and nothing is zeroed
-// beforehand (no counter, no atomics: sums are formed in a fixed order, in double, since what is left after
-// advantages of both signs cancel is small beside the terms).
+// first block joins: no second launch), then (backward) one pass that writes the gradient.  A token costs 9 to 21 bytes and
+// a few dozen operations, so long batches are bound by HBM and arithmetic, the usual ones by launches.  Nothing is zeroed
+// beforehand (no counter, no atomics): sums are formed in a fixed order, and in double, since what is left after advantages
+// of both signs cancel is small beside the terms.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -561,8 +561,8 @@ int check_workspace(const b200tp_objective_args* a, void* workspace, size_t byte
   return B200TP_OK;
 }
 
-// A tokens kernel and its join: one launch of a cluster of 2, 4 or 8 blocks where that holds them all (8 x 61 tokens, forward and backward: 6.5 us on the
-// device against 7.8, and 2 us less of host time), else two launches.
+// A tokens kernel and its join: one launch of a cluster of 1, 2, 4 or 8 blocks where that holds them all (8 x 61 tokens, forward and
+// backward: 6.5 us on the device against 7.8, and 2 us less of host time), else two launches.
 template <typename Join, typename Go>
 int launch_both(unsigned blocks, const Part* parts, const Tokens& t, const Join& o, cudaStream_t stream, Go go) {
   if (blocks <= kClusterMost) {
