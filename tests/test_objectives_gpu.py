@@ -443,6 +443,25 @@ def test_other_stream_and_captured(cuda_device):
         assert torch.equal(out[0], want[k][0]) and torch.equal(out[1], want[k][1])
 
 
+def test_offsets_beyond_32_bits(cuda_device):
+    """More than 2^31 tokens, rows of up to 2^30 (the longest), and packed: every token's slope is the same, at the ends too."""
+    dev = cuda_device
+    for seqs, length in ((3, 1 << 30), (4, (1 << 29) + 5)):
+        x = torch.zeros(seqs, length, dtype=torch.bfloat16, device=dev, requires_grad=True)
+        a = torch.arange(1.0, seqs + 1, device=dev)[:, None]
+        out = policy_loss(x, torch.zeros_like(x), a, normalize="sequence")
+        grad, = torch.autograd.grad(out.loss, x)
+        assert abs(out.loss.item() + a.mean().item()) <= 1e-6 * a.mean().item()
+        want = (-a[:, 0].double() / (seqs * length))
+        for at in (0, 1, length // 2, length - 1):
+            assert ((grad[:, at].double() - want).abs() <= 2.0 ** -7 * want.abs()).all()
+        del grad, out
+    loss = preference_loss(x, beta=1.0)
+    grad, = torch.autograd.grad(loss.loss, x)
+    assert abs(loss.loss.item() - math.log(2)) < 1e-6
+    assert (grad[:2, [0, length - 1]] == -0.25).all() and (grad[2:, [0, length - 1]] == 0.25).all()
+
+
 def test_refusals(cuda_device):
     dev = cuda_device
     x = torch.zeros(4, 8, device=dev)
