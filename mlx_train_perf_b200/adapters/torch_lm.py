@@ -66,11 +66,11 @@ def split_model(model: Any) -> tuple[Callable[[torch.Tensor], torch.Tensor], Hea
 def _trains_plain_table(mod: Any) -> bool:
     """Whether `embed_tokens` is a plain nn.Embedding with a trained fp32 / bf16 table on a GPU and nothing attached to it: then
     `embedding_lookup` gives the same rows and the same gradient (summed in fp32 in a fixed order, rounded once).  Anything
-    else (frozen, wrapped by an adapter, hooked, norm-limited, sparse) stays the module's own."""
+    else (frozen, wrapped by an adapter, hooked, sharded, norm-limited, sparse) stays the module's own."""
     if type(mod) is not torch.nn.Embedding or not torch.is_grad_enabled() or _has_any_global_hook():
         return False
     w = mod.weight
-    return (isinstance(w, torch.Tensor) and w.is_cuda and w.requires_grad and w.dtype in (torch.float32, torch.bfloat16)
+    return (type(w) in (torch.Tensor, torch.nn.Parameter) and w.is_cuda and w.requires_grad and w.dtype in (torch.float32, torch.bfloat16)
             and mod.max_norm is None and not mod.sparse and not mod.scale_grad_by_freq
             and not torch.is_autocast_enabled("cuda")
             and not (mod._forward_hooks or mod._forward_pre_hooks or mod._backward_hooks or mod._backward_pre_hooks))

@@ -144,6 +144,12 @@ def test_which_tables_the_walk_looks_up(cuda_device):
         assert not torch_lm._trains_plain_table(other.to(cuda_device))
     assert not torch_lm._trains_plain_table(torch.nn.Embedding(10, 8))
 
+    class Sharded(torch.Tensor):
+        pass
+
+    mod.weight = torch.nn.Parameter(torch.zeros(10, 8, device=cuda_device).as_subclass(Sharded))
+    assert isinstance(mod.weight, Sharded) and not torch_lm._trains_plain_table(mod)
+
 
 @pytest.mark.gpu
 def test_planner_measures_with_the_package_optimizer(cuda_device):
