@@ -39,10 +39,11 @@ def _look_up(weight: torch.Tensor, ids: torch.Tensor, scale: float, padding: int
 
 
 class _Lookup(torch.autograd.Function):
-    """(weight, ids, scale, padding) -> ids.shape + (D,)."""
+    """(weight, (ids, scale, padding)) -> ids.shape + (D,)."""
 
     @staticmethod
-    def forward(ctx, weight, ids, scale, padding):
+    def forward(ctx, weight, call):
+        ids, scale, padding = call
         ctx.save_for_backward(ids)
         ctx.rule = *weight.shape, weight.dtype, scale, padding
         return _look_up(weight, ids, scale, padding)
@@ -68,7 +69,7 @@ class _Lookup(torch.autograd.Function):
             rc = lib.b200tp_embedding_bwd(C.byref(a), rows.data_ptr(), grad.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
                                           _lib.stream(dev), device_status(dev).data_ptr())
         _lib.check(rc)
-        return grad, None, None, None
+        return grad, None
 
 
 def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, padding_idx: int | None = None,
@@ -78,20 +79,20 @@ def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 
     ids: integers of any shape on the table's device (int32 and int64 are read as they are).  `padding_idx`: that row gets no gradient.  An id
     outside [0, V) gives a row of zeros and no gradient, and `core.loss.check_device_status()` reports it; `validate_ids=True`
     raises before the launch, with a host synchronisation.  The gradient is dense (V, D)."""
-    if weight.ndim != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise EmbeddingInputError(f"weight must be (V, D), got {tuple(weight.shape)}")
+    shape = weight.shape
+    if len(shape) != 2 or 0 in shape:
+        raise EmbeddingInputError(f"weight must be (V, D), got {tuple(shape)}")
     if not weight.is_cuda:
         raise EmbeddingInputError(f"weight must be a CUDA tensor (the operator has no CPU path); got {weight.device}")
     if weight.dtype not in _DTYPES:
         raise EmbeddingInputError(f"weight must be fp32 or bf16, got {weight.dtype}")
-    if ids.device != weight.device:
+    if ids.get_device() != weight.get_device():
         raise EmbeddingInputError(f"ids are on {ids.device}, weight on {weight.device}")
     if ids.dtype not in (torch.int64, torch.int32):
         if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
             raise EmbeddingInputError(f"ids must be an integer dtype, got {ids.dtype}")
         ids = ids.to(torch.int64)
-    v, d = weight.shape
-    padding = -1
+    v, padding = shape[0], -1
     if padding_idx is not None:
         if not -v <= padding_idx < v:
             raise EmbeddingInputError(f"padding_idx must lie in [-{v}, {v}), got {padding_idx}")
@@ -103,5 +104,5 @@ def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 
     if not ids.is_contiguous():
         ids = ids.contiguous()
     if weight.requires_grad and torch.is_grad_enabled():
-        return _Lookup.apply(weight, ids, float(scale), padding)
+        return _Lookup.apply(weight, (ids, float(scale), padding))
     return _look_up(weight, ids, float(scale), padding)     # without autograd's function around it: 6 us of some 17
