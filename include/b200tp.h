@@ -422,7 +422,7 @@ typedef struct b200tp_adamw_args {
 
 /* m = b1 m + (1 - b1) g; v = b2 v + (1 - b2) g g; p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps), in
  * fp32, each stored value rounded once.  `tensors` is host memory, read before the call returns; up to 600 tensors a
- * launch.  Tensors that share memory are refused. */
+ * launch.  Tensors that share memory are refused; a gradient may only be the very memory that its own param_out is. */
 int b200tp_adamw_step(const b200tp_adamw_args* a, const b200tp_adamw_tensor* tensors, int32_t count, void* stream);
 
 /* Writes the addresses of `count` Python tensor objects into column 0 (param), 1 (grad) or 2 (param_out) of `rows`.  describe: the

@@ -209,8 +209,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
     else:
         for k, i in enumerate(which):
             out_state.steps[i] = int(step) if steps is None else steps[k]
-    if out is None:
-        increment_version([params[i] for i in which])    # autograd is told that saved copies are stale
+    increment_version(out_params if len(which) == len(params) else [out_params[i] for i in which])    # autograd is told that saved copies are stale
 
 
 class _Bucket:

@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <iterator>
 #include <type_traits>
 #include <vector>
 
@@ -463,8 +464,9 @@ int launch_kind(const b200tp_adamw_args* a, const b200tp_adamw_tensor* t, int co
 bool misaligned(const void* p, unsigned mask) { return (reinterpret_cast<uintptr_t>(p) & mask) != 0; }
 
 // Written ranges that overlap, or overlap what another tensor's step reads, would race: the same tensor twice, views of one another, an
-// output over another tensor's input.
-int check_apart(std::vector<std::pair<uintptr_t, uintptr_t>>& ranges, const char* what) {
+// output over another tensor's input or gradient.
+using Ranges = std::vector<std::pair<uintptr_t, uintptr_t>>;
+int check_apart(Ranges& ranges, const char* what) {
   std::sort(ranges.begin(), ranges.end());
   for (size_t i = 1; i < ranges.size(); ++i)
     if (ranges[i].first < ranges[i - 1].second)
@@ -490,8 +492,8 @@ int check(const b200tp_adamw_args* a, const b200tp_adamw_tensor* t, int32_t coun
   const void* states[] = {a->exp_avg, a->exp_avg_sq, a->scales, a->master, a->exp_avg_out, a->exp_avg_sq_out, a->scales_out, a->master_out};
   for (const void* p : states)
     if (misaligned(p, 15)) return fail(B200TP_ERR_OPTIM_INPUT, "states must be 16-byte aligned");
-  std::vector<std::pair<uintptr_t, uintptr_t>> written, offsets;
-  written.reserve(2 * count);
+  Ranges outs, inputs, offsets;
+  outs.reserve(count);
   offsets.reserve(count);
   const unsigned p_item = a->param_dtype == B200TP_BF16 ? 2 : 4, g_item = a->grad_dtype == B200TP_BF16 ? 2 : 4;
   for (int i = 0; i < count; ++i) {
@@ -503,12 +505,26 @@ int check(const b200tp_adamw_args* a, const b200tp_adamw_tensor* t, int32_t coun
     if (t[i].state_offset < 0 || t[i].state_offset % kBlock != 0)
       return fail(B200TP_ERR_OPTIM_INPUT, "a tensor's place in the states must be a multiple of 256 elements");
     const uintptr_t p = reinterpret_cast<uintptr_t>(t[i].param_out), q = reinterpret_cast<uintptr_t>(t[i].param);
-    written.emplace_back(p, p + static_cast<uintptr_t>(t[i].numel) * p_item);
-    if (q != p && a->master == nullptr) written.emplace_back(q, q + static_cast<uintptr_t>(t[i].numel) * p_item);   // read by others
+    outs.emplace_back(p, p + static_cast<uintptr_t>(t[i].numel) * p_item);
+    if (q != p && a->master == nullptr) inputs.emplace_back(q, q + static_cast<uintptr_t>(t[i].numel) * p_item);
     offsets.emplace_back(t[i].state_offset, t[i].state_offset + align_up(t[i].numel, kBlock));
   }
-  const int rc = check_apart(written, "parameters");
-  return rc ? rc : check_apart(offsets, "states");
+  int rc = check_apart(outs, "parameters");
+  if (rc) return rc;
+  for (int i = 0; i < count; ++i) {           // a gradient may lie where its own results go, element on element
+    if (t[i].numel == 0) continue;
+    const uintptr_t g = reinterpret_cast<uintptr_t>(t[i].grad), end = g + static_cast<uintptr_t>(t[i].numel) * g_item;
+    if (t[i].grad == t[i].param_out && g_item == p_item) continue;
+    const auto next = std::lower_bound(outs.begin(), outs.end(), std::make_pair(end, uintptr_t{0}));    // begins behind it
+    if (next != outs.begin() && std::prev(next)->second > g)
+      return fail(B200TP_ERR_OPTIM_INPUT, "two tensors of one step share memory (a gradient and a parameter)");
+  }
+  if (!inputs.empty()) {
+    inputs.insert(inputs.end(), outs.begin(), outs.end());
+    rc = check_apart(inputs, "parameters");
+    if (rc) return rc;
+  }
+  return check_apart(offsets, "states");
 }
 
 }  // namespace

@@ -136,6 +136,26 @@ def test_other_buffers_get_what_the_step_in_place_gives(cuda_device, bits, maste
     assert all(torch.equal(getattr(state, n).view(torch.uint8), getattr(after, n).view(torch.uint8)) for n in names)
 
 
+def test_other_buffers_are_known_to_have_changed(cuda_device):
+    """A graph that saved an output's old value must not use the new one."""
+    p, to = torch.ones(300, device=cuda_device), torch.ones(300, device=cuda_device, requires_grad=True)
+    loss = to.square().sum()
+    adamw_step([p], [p.clone()], AdamWState.zeros([p]), out=([to], AdamWState.zeros([p])), **RULE)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_gradient_that_its_own_result_replaces(cuda_device, bits):
+    dev = cuda_device
+    params, grads = _tensors(SHAPES, torch.bfloat16, dev, 3), _tensors(SHAPES, torch.bfloat16, dev, 4)
+    one, two = AdamWState.zeros(params, bits=bits), AdamWState.zeros(params, bits=bits)
+    over = [g.clone() for g in grads]
+    adamw_step(params, over, one, out=(over, two), **RULE)
+    adamw_step(params, grads, one, **RULE)
+    assert all(torch.equal(p, q) for p, q in zip(params, over))
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_unaligned_views_and_strided_gradients(cuda_device, bits):
     """Parameters and gradients one element off an aligned address, odd sizes, gradients transposed: the values of aligned ones."""

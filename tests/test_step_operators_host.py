@@ -90,6 +90,25 @@ def test_adamw_tables(lib, rows):
     assert _adamw(rows) == _lib.ERR_OPTIM_INPUT
 
 
+@pytest.mark.parametrize("rows,change", [
+    ([[PTR, PTR + 8, PTR, 100, 0]], {}), ([[PTR, PTR + 4096, PTR, 100, 0], [PTR + 8192, PTR, PTR + 8192, 100, 256]], {}),
+    ([[PTR, PTR + 396, PTR, 100, 0]], {}), ([[PTR + 400, PTR + 4, PTR + 400, 100, 0]], {}), ([[PTR, PTR, PTR, 100, 0]], dict(grad_dtype=1)),
+    ([[PTR, PTR + 64, PTR + 4096, 100, 0], [PTR + 400, PTR + 4200, PTR + 8192, 100, 256]], {})])
+def test_gradients_in_the_way_of_results(lib, rows, change):
+    """A gradient that another tensor's results, or its own ones elsewhere, would overwrite while it is read."""
+    assert _adamw(rows, **change) == _lib.ERR_OPTIM_INPUT and b"a gradient and a parameter" in lib.b200tp_last_error()
+
+
+@pytest.mark.parametrize("rows", [
+    [[PTR, PTR, PTR, 100, 0]], [[PTR, PTR + 400, PTR, 100, 0]], [[PTR + 400, PTR, PTR + 400, 100, 0]], [[PTR, PTR, PTR + 4096, 100, 0]],
+    [[PTR, PTR + 4096, PTR + 4096, 100, 0]], [[PTR, PTR + 4096, PTR, 100, 0], [PTR + 400, PTR + 4096, PTR + 400, 100, 256]]])
+def test_gradients_that_are_in_no_way(lib, rows):
+    """Beside the results, exactly on them, on read-only parameters, and one gradient for two tensors: the tensors pass, and what is refused
+    is the table behind them, whose place in the states is the first one's."""
+    assert _adamw(rows + [[PTR + (1 << 16), PTR + (1 << 17), PTR + (1 << 16), 100, 0]]) == _lib.ERR_OPTIM_INPUT
+    assert b"(states)" in lib.b200tp_last_error()
+
+
 def test_addresses_of_many_tensors(lib):
     """The DLPack table of this torch, on host tensors: addresses of row-major tensors of the type and size, the first other one's index."""
     fn = _lib.tensor_rows()
