@@ -160,10 +160,11 @@ __device__ __forceinline__ float rcp_ftz(float v) {
   return q;
 }
 
-// 448 / v, with a Newton step behind the approximate reciprocal: all codes of a block depend on it.
+// 448 / v to half an ulp: the product with an approximate reciprocal, corrected by its exact remainder.  All codes of a block depend on
+// it.  (The reciprocal with a Newton step and then times 448 is two roundings.)
 __device__ __forceinline__ float over(float v) {
-  const float q = rcp_ftz(v);
-  return 448.f * fmaf(fmaf(-v, q, 1.f), q, q);
+  const float q = rcp_ftz(v), x = 448.f * q;
+  return fmaf(fmaf(-v, x, 448.f), q, x);
 }
 constexpr float kNoRoot = 4e-19f;           // roots up to here stand for zero: the root of 1e-37 is 3.2e-19
 

@@ -249,6 +249,29 @@ def test_tensors_asked_one_by_one(cuda_device, monkeypatch):
     assert all(torch.equal(a, b) for a, b in zip(params, want))
 
 
+def test_8_bit_codes_are_off_by_two_roundings_at_most(cuda_device):
+    """m as a code is m * (448 / largest), each of the two rounded once: where the exact quotient is farther than 2 x 2^-24 of itself
+    (and what the two multiply to, 2^-6 of that) from the middle between two codes, the code is the nearest one.  With betas of 0
+    the first step's m are the gradients themselves, placed around such middles here."""
+    dev = cuda_device
+    g = torch.Generator().manual_seed(31)
+    blocks = 8192
+    top = 1 + torch.rand(blocks, 1, generator=g)
+    middle = (torch.randint(8, 15, (blocks, 256), generator=g) + 0.5) * 2.0 ** torch.randint(-8, 5, (blocks, 256), generator=g)
+    near = 1 + torch.randint(-64, 65, (blocks, 256), generator=g).double() / 16 * E32
+    grad = (middle.double() * near * top.double() / 448).float()
+    grad[:, :1] = top
+    p = [torch.zeros(blocks * 256, device=dev)]
+    state = AdamWState.zeros(p, bits=8)
+    adamw_step(p, [grad.reshape(-1).to(dev)], state, lr=0.0, betas=(0.0, 0.0))
+    got = state.exp_avg.cpu().float().double().reshape(blocks, 256)[:, 1:]
+    y, middle = (grad.double() * 448 / top.double())[:, 1:], middle.double()[:, 1:]
+    nearest = torch.round(y / _e4m3_step(y)) * _e4m3_step(y)
+    clear = (y / middle - 1).abs() > 2 * E32 * (1 + 2.0 ** -6)
+    assert 0.3 < clear.double().mean() < 0.7
+    assert torch.equal(got[clear], nearest[clear])
+
+
 def test_8_bit_roots_are_rounded_without_drift(cuda_device):
     """A million equal roots between two codes: the mean of the codes is the root, up to five standard errors and the dither's own
     2^-17 of a step; and a v that is not zero never becomes zero, whatever the block's largest."""
