@@ -8,8 +8,9 @@ The reference trains with `mlx.optimizers.AdamW`, and its planner books two fp32
 
 `adamw_step` is that step on lists of tensors, in place or into other buffers; `AdamW` is the `torch.optim.Optimizer` a trainer
 holds.  8-bit moments take 2 bytes a parameter and 8 for every 256: e4m3 codes of m and of sqrt(v) times a scale for each
-block of 256 elements; sqrt(v) is rounded up or down by a dither fixed by position and step, so every rank of a
-data-parallel run gets the same codes.
+block of 256 elements; sqrt(v), and m wherever rounding to nearest could hold a value that no gradient feeds (small codes; with
+beta1 above 0.9 all of them), is rounded up or down by a dither fixed by position and step, so every rank of a data-parallel run gets
+the same codes.
 """
 from __future__ import annotations
 

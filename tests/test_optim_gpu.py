@@ -300,6 +300,89 @@ def test_8_bit_roots_are_rounded_without_drift(cuda_device):
     assert (v[:, 1] == 0).all() and (v[:, 2:] > 0).all() and (v[:, 0] > 0).all()
 
 
+@pytest.mark.parametrize("beta1,code", [(0.9, 4), (0.9, -4), (0.9, 1), (0.95, 9), (0.95, -9), (0.99, 8), (0.99, 300), (0.95, 3)])
+def test_8_bit_m_that_nothing_feeds_is_not_held(cuda_device, beta1, code):
+    """Half a million equal m without a gradient, each a code (in units of 2^-9 up to 7, of 2^-6 / 8 ... above) that rounding to nearest
+    would bring back: after a step their mean is beta1 times the code, up to five standard errors, the dither's own 2^-17 of a
+    distance and the roundings of m and of its scale."""
+    dev = cuda_device
+    n = 256 * 2048
+    y = torch.tensor(code / 512.0).to(torch.float8_e4m3fn).float().item()
+    m = torch.full((n,), y, device=dev)
+    m[::256] = 448.0
+    state = AdamWState([n], m.to(torch.float8_e4m3fn), torch.full((n,), 1.0, device=dev).to(torch.float8_e4m3fn),
+                       scales=torch.ones(n // 256, 2, device=dev), steps=[200])
+    g = torch.zeros(n, device=dev)
+    g[::256] = 448.0                                              # holds the scale
+    adamw_step([torch.zeros(n, device=dev)], [g], state, lr=0.0, betas=(beta1, 0.999))
+    got = state.moments(0)[0].double().reshape(-1, 256)[:, 1:]
+    step = _e4m3_step(torch.tensor(y)).item()
+    se = step / 2 / math.sqrt(got.numel())
+    assert 1 <= got.unique().numel() <= 2 and got.unique().abs().min() < abs(y)
+    assert abs(got.mean().item() - beta1 * y) < 5 * se + step * 2.0 ** -17 + abs(y) * 8 * E32
+
+
+@pytest.mark.parametrize("betas,steps", [((0.9, 0.999), 4000), ((0.9, 0.95), 3000), ((0.95, 0.95), 3000), ((0.95, 0.999), 3000)])
+def test_8_bit_parameters_stop_where_gradients_do(cuda_device, betas, steps):
+    """Twenty steps with gradients of 0.5, then none, while the block's largest stays at 1: a parameter moves as far as in 64 bits.  What may
+    differ: m rounded to nearest falls by at least two thirds of what it should a step (code 15 goes to 14 and not to 13.5, 14
+    to 13 and not to 12.6), dithered m by as much in the mean; 1 / sqrt(v) is up to 1.18 times too large in the mean (a
+    root's dither has a variance of at most (1/8)^2 / 4 a step, weighed with the decay of m / sqrt(v), 0.975 a step at the
+    slowest).  So 0.95 to 1.8 times; m is zero at the end (beta1^t is below 1e-60), and nothing moves any more."""
+    dev = cuda_device
+    n = 256 * 64
+    p, state = [torch.zeros(n, device=dev)], AdamWState.zeros([torch.zeros(n, device=dev)], bits=8)
+    hot = torch.zeros(n, device=dev)
+    hot[::256] = 1.0
+    fed = torch.where(hot > 0, 1.0, 0.5)
+    want = m = v = 0.0
+    for t in range(1, steps + 1):
+        g = 0.5 if t <= 20 else 0.0
+        m, v = betas[0] * m + (1 - betas[0]) * g, betas[1] * v + (1 - betas[1]) * g * g
+        want += m / (1 - betas[0] ** t) / math.sqrt(v / (1 - betas[1] ** t)) if v > 0 else 0.0
+        adamw_step(p, [fed if t <= 20 else hot], state, lr=1.0, betas=betas, eps=0.0, weight_decay=0.0)
+    rest = hot == 0
+    moved = -p[0][rest].double()
+    assert 0.95 * want < moved.mean().item() < 1.8 * want, (moved.mean().item(), want)
+    assert (state.moments(0)[0][rest] == 0).all()
+    before = p[0].clone()
+    adamw_step(p, [hot], state, lr=1.0, betas=betas, eps=0.0, weight_decay=0.0)
+    assert torch.equal(p[0][rest], before[rest])
+
+
+def test_8_bit_m_with_a_large_beta1(cuda_device):
+    """Above 0.9 every m is dithered: a million equal m between two codes have the right mean, a block's largest stays the largest code,
+    other steps give other codes, and what is not finite is NaN and leaves its block alone."""
+    dev = cuda_device
+    n = 1 << 20
+    p = [torch.zeros(n, device=dev)]
+    for sign in (1.0, -1.0):
+        g = torch.full((n,), 1.3 * sign, device=dev)
+        g[::256] = 7.0 * sign
+        state = AdamWState.zeros(p, bits=8)
+        adamw_step(p, [g], state, lr=0.0, betas=(0.95, 0.999))
+        m = state.moments(0)[0].double().reshape(-1, 256) * sign / 0.05
+        step = 2.0 ** (math.floor(math.log2(1.3 / (7.0 / 448))) - 3) * 7.0 / 448
+        assert m[:, 1:].unique().numel() == 2 and (m[:, 0] - 7.0).abs().max() < 7 * 8 * E32
+        assert abs(m[:, 1:].mean().item() - 1.3) < 5 * step / 2 / math.sqrt(m[:, 1:].numel()) + step * 2.0 ** -17 + 1.3 * 8 * E32
+    first = state.exp_avg.view(torch.uint8).clone()
+    again = AdamWState.zeros(p, bits=8)
+    adamw_step(p, [g], again, lr=0.0, betas=(0.95, 0.999))
+    assert torch.equal(again.exp_avg.view(torch.uint8), first)
+    again = AdamWState.zeros(p, bits=8)
+    adamw_step(p, [g], again, lr=0.0, betas=(0.95, 0.999), step=2)
+    assert not torch.equal(again.exp_avg.view(torch.uint8), first)
+    bad = g.clone()
+    bad[5], bad[300], bad[777] = math.nan, math.inf, -math.inf
+    voided = torch.zeros(n, dtype=torch.bool, device=dev)
+    voided[[5, 300, 777]] = True
+    got = AdamWState.zeros(p, bits=8)
+    adamw_step([p[0].clone()], [bad], got, lr=0.0, betas=(0.95, 0.999))
+    m, v = got.moments(0)
+    assert torch.isnan(m[voided]).all() and torch.isnan(v[voided]).all()
+    assert torch.equal(got.exp_avg.view(torch.uint8)[~voided], first[~voided])
+
+
 def test_8_bit_moments_follow_a_falling_gradient(cuda_device):
     """Gradients of one element fall to zero while its block's largest stays: rounding to nearest would hold its root for ever
     (a step changes it by 0.05 %, half a code's distance is 3 %); after 3000 steps with b2 = 0.999 it has shrunk to exp(-1.5)
