@@ -239,30 +239,40 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, {"lr": lr, "betas": tuple(betas), "eps": eps, "weight_decay": weight_decay})
 
     def _of_group(self, k: int) -> list[_Bucket]:
+        """The group's buckets, laid out at the first call with what `self.state` holds; kept only once all of it fits."""
         if k not in self._buckets:
             kinds: dict[Any, list[torch.Tensor]] = {}
             for p in self.param_groups[k]["params"]:
                 kinds.setdefault((p.dtype, p.device), []).append(p)
-            self._buckets[k] = [_Bucket(ps, self._bits, self._master) for ps in kinds.values()]
-            for b in self._buckets[k]:
+            buckets, states = [_Bucket(ps, self._bits, self._master) for ps in kinds.values()], {}
+            for b in buckets:
                 for i, p in enumerate(b.params):
                     saved = self.state.get(p)
                     if saved:
-                        self._restore(b, i, saved)
-                    self.state[p] = {"step": b.state.steps[i], **{name: b.state.view(name, i) for name in b.names()}}
+                        self._check_saved(p, saved)
+                        for name in b.names():
+                            b.state.view(name, i).copy_(saved[name])
+                        b.state.steps[i] = int(saved["step"])
+                    states[p] = {"step": b.state.steps[i], **{name: b.state.view(name, i) for name in b.names()}}
+            self.state.update(states)
+            self._buckets[k] = buckets
         return self._buckets[k]
 
-    @staticmethod
-    def _restore(b: _Bucket, i: int, saved: dict) -> None:
-        if set(saved) != {"step", *b.names()}:
-            raise OptimizerInputError(f"a saved state has {sorted(saved)}, this optimizer keeps {sorted(['step', *b.names()])}")
-        for name in b.names():
-            to = b.state.view(name, i)
-            if saved[name].shape != to.shape or saved[name].dtype != to.dtype:
-                raise OptimizerInputError(f"{name} of a saved state is {tuple(saved[name].shape)} {saved[name].dtype}, not "
-                                          f"{tuple(to.shape)} {to.dtype}")
-            to.copy_(saved[name])
-        b.state.steps[i] = int(saved["step"])
+    def _check_saved(self, p: torch.Tensor, saved: dict) -> None:
+        """Whether a saved state is one that this optimizer keeps for `p`."""
+        n, moments = p.numel(), torch.float32 if self._bits == 32 else torch.float8_e4m3fn
+        kept = {"exp_avg": ((n,), moments), "exp_avg_sq": ((n,), moments)}
+        if self._bits == 8:
+            kept["scales"] = ((_padded(n) // BLOCK, 2), torch.float32)
+        if self._master and p.dtype == torch.bfloat16:
+            kept["master"] = ((n,), torch.float32)
+        if set(saved) != {"step", *kept}:
+            raise OptimizerInputError(f"a saved state has {sorted(saved)}, this optimizer keeps {sorted(['step', *kept])}")
+        for name, (shape, dtype) in kept.items():
+            if tuple(saved[name].shape) != shape or saved[name].dtype != dtype:
+                raise OptimizerInputError(f"{name} of a saved state is {tuple(saved[name].shape)} {saved[name].dtype}, not {shape} {dtype}")
+        if int(saved["step"]) < 0:
+            raise OptimizerInputError(f"a saved state has taken {int(saved['step'])} steps")
 
     @torch.no_grad()
     def step(self, closure=None, *, grad_scale: float | torch.Tensor = 1.0):
@@ -289,14 +299,17 @@ class AdamW(torch.optim.Optimizer):
         return super().state_dict()
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """Hyperparameters and states as saved, in their own dtypes (the base class would cast moments to the parameters')."""
-        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        """Hyperparameters and states as saved, in their own dtypes (the base class would cast moments to the parameters').  A saved
+        state that does not fit is refused before anything is changed."""
         order = [p for group in self.param_groups for p in group["params"]]
         names = [i for group in state_dict["param_groups"] for i in group["params"]]
+        saved = {p: state_dict["state"][name] for name, p in zip(names, order) if name in state_dict["state"]}
+        for p, of_p in saved.items():
+            self._check_saved(p, of_p)
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})     # refuses other groups than these
         self._buckets = {}
-        for name, p in zip(names, order):
-            if name in state_dict["state"]:
-                self.state[p] = dict(state_dict["state"][name])
+        for p, of_p in saved.items():
+            self.state[p] = dict(of_p)
         for k in range(len(self.param_groups)):
             self._of_group(k)
 

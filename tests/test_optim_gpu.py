@@ -540,6 +540,39 @@ def test_saved_and_loaded_optimizer_goes_on_alike(cuda_device, bits, master):
         AdamW(b.parameters(), bits=40 - bits, master=master).load_state_dict(saved["opt"])
 
 
+@pytest.mark.parametrize("bits,master", [(32, False), (8, True)])
+def test_a_refused_load_changes_nothing(cuda_device, bits, master):
+    """Saved states that do not fit, the last parameter's alone among them: refused, and training goes on bit for bit as without them."""
+    dtype = torch.bfloat16 if master else torch.float32
+    a = _model(cuda_device, dtype)
+    groups = [{"params": a[0].parameters()}, {"params": a[2].parameters(), "lr": 3e-3}]
+    opt = AdamW(groups, lr=1e-2, bits=bits, master=master)
+    _train(a, opt, 3)
+    b, twin = copy.deepcopy((a, opt))
+    good = copy.deepcopy(opt.state_dict())
+    good["param_groups"][0]["lr"] = 7.0
+    last = max(good["state"])
+    for spoil in (lambda d: d["state"][last].pop("exp_avg_sq"), lambda d: d["state"][last].update(more=torch.zeros(1)),
+                  lambda d: d["state"][last].update(exp_avg=d["state"][0]["exp_avg"]), lambda d: d["state"][last].update(step=-1),
+                  lambda d: d["state"][last].update(exp_avg=d["state"][last]["exp_avg"].to(torch.float16)),
+                  lambda d: d["state"].update({k: {**v, "exp_avg": v["exp_avg"].double()} for k, v in d["state"].items()}),
+                  lambda d: d["param_groups"].pop(), lambda d: d["param_groups"][1]["params"].pop()):
+        bad = copy.deepcopy(good)
+        spoil(bad)
+        with pytest.raises((OptimizerInputError, ValueError)):
+            opt.load_state_dict(bad)
+        assert opt.param_groups[0]["lr"] == 1e-2
+    for m, o in ((a, opt), (b, twin)):
+        _train(m, o, 2, seed=3)
+    assert all(torch.equal(p, q) for p, q in zip(a.parameters(), b.parameters()))
+    one, two = opt.state_dict(), twin.state_dict()
+    assert all(s["step"] == 5 for s in one["state"].values())
+    assert all(torch.equal(one["state"][k][n].view(torch.uint8), two["state"][k][n].view(torch.uint8))
+               for k in one["state"] for n in one["state"][k] if n != "step")
+    opt.load_state_dict(good)                                     # and the one that fits still loads
+    assert opt.param_groups[0]["lr"] == 7.0 and all(s["step"] == 3 for s in opt.state_dict()["state"].values())
+
+
 def test_mixed_dtypes_missing_gradients_and_versions(cuda_device):
     dev = cuda_device
     p = [torch.nn.Parameter(t) for t in (torch.ones(10, device=dev), torch.ones(300, device=dev, dtype=torch.bfloat16), torch.ones(7, device=dev))]
