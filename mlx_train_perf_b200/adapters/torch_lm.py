@@ -63,11 +63,17 @@ def split_model(model: Any) -> tuple[Callable[[torch.Tensor], torch.Tensor], Hea
     return trunk, head
 
 
+_EMBEDDING_FORWARD = torch.nn.Embedding.forward
+
+
 def _trains_plain_table(mod: Any) -> bool:
     """Whether `embed_tokens` is a plain nn.Embedding with a trained fp32 / bf16 table on a GPU and nothing attached to it: then
     `embedding_lookup` gives the same rows and the same gradient (summed in fp32 in a fixed order, rounded once).  Anything
-    else (frozen, wrapped by an adapter, hooked, sharded, norm-limited, sparse) stays the module's own."""
+    else (frozen, wrapped by an adapter, hooked, with a `forward` put in place of its own, sharded, norm-limited, sparse) stays the
+    module's own."""
     if type(mod) is not torch.nn.Embedding or not torch.is_grad_enabled() or _has_any_global_hook():
+        return False
+    if "forward" in vars(mod) or torch.nn.Embedding.forward is not _EMBEDDING_FORWARD:
         return False
     w = mod.weight
     return (type(w) in (torch.Tensor, torch.nn.Parameter) and w.is_cuda and w.requires_grad and w.dtype in (torch.float32, torch.bfloat16)

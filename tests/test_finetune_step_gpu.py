@@ -152,6 +152,30 @@ def test_which_tables_the_walk_looks_up(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("where", ["instance", "class"])
+def test_a_forward_put_in_place_of_the_table_s_own(cuda_device, monkeypatch, where):
+    """As tools that wrap modules in place do it: the walk's rows are that function's, and so is the table's gradient."""
+    dev = cuda_device
+    stock, ours = _pair(dev)
+    batch, lengths = _batch(dev)
+    own = torch.nn.Embedding.forward
+    if where == "class":
+        monkeypatch.setattr(torch.nn.Embedding, "forward", lambda self, ids: 3.0 * own(self, ids) + 0.01)
+    else:
+        for model in (stock, ours):
+            table = model.model.embed_tokens
+            table.forward = lambda ids, table=table: 3.0 * own(table, ids) + 0.01
+    assert not torch_lm._trains_plain_table(ours.model.embed_tokens)
+    got, _ = make_loss_fn(ours)(ours, batch, lengths)
+    x, mask = _plain_logps(stock, batch, lengths)
+    want = -(x * mask).sum() / mask.sum()
+    got.backward()
+    want.backward()
+    assert abs(got.item() - want.item()) < 1e-4 * max(1.0, abs(want.item()))
+    _gradients_agree(ours, stock)
+
+
+@pytest.mark.gpu
 def test_planner_measures_with_the_package_optimizer(cuda_device):
     """One small point of the planner's measuring command, moments of either width: 8 bits take less, and both run."""
     from mlx_train_perf_b200.plan import estimate as E
