@@ -9,8 +9,8 @@ the flash wrapper refuses), then feed the hidden states to the fused loss with t
 materialised.  Masked mean: loss = sum(nll * mask) / ntoks, reduced inside the library.
 
 `make_token_loss_fn` stops before that reduction; `make_preference_loss_fn` and `make_policy_loss_fn` go on from the
-per-token losses with the objectives of `core/objectives.py`.  Where the embedding table is trained, the walk looks rows
-up with `embedding_lookup`, whose gradient adds the rows of equal ids in a fixed order.
+per-token losses with the objectives of `core/objectives.py`.  Where the embedding table is trained, its gradient is
+`embedding_lookup`'s, which adds the rows of equal ids in a fixed order.
 """
 from __future__ import annotations
 
@@ -21,7 +21,7 @@ from torch.nn.modules.module import _has_any_global_hook
 
 from mlx_train_perf_b200.attention.segments import PackedMask
 from mlx_train_perf_b200.attention.wrapper import SUPPORTED_FAMILIES, FlashAttentionWrapper
-from mlx_train_perf_b200.core.embedding import embedding_lookup
+from mlx_train_perf_b200.core.embedding import module_lookup
 from mlx_train_perf_b200.core.loss import (IGNORE_INDEX, DenseHead, HeadRef, QuantizedHead, fused_linear_ce,
                                            reduced_linear_cross_entropy, resolve_impl, tied_head)
 from mlx_train_perf_b200.core.objectives import PolicyLoss, PreferenceLoss, policy_loss, preference_loss
@@ -68,7 +68,7 @@ _EMBEDDING_FORWARD = torch.nn.Embedding.forward
 
 def _trains_plain_table(mod: Any) -> bool:
     """Whether `embed_tokens` is a plain nn.Embedding with a trained fp32 / bf16 table on a GPU and nothing attached to it: then
-    `embedding_lookup` gives the same rows and the same gradient (summed in fp32 in a fixed order, rounded once).  Anything
+    `embedding_lookup` gives the same gradient (summed in fp32 in a fixed order, rounded once).  Anything
     else (frozen, wrapped by an adapter, hooked, with a `forward` put in place of its own, sharded, norm-limited, sparse) stays the
     module's own."""
     if type(mod) is not torch.nn.Embedding or not torch.is_grad_enabled() or _has_any_global_hook():
@@ -84,8 +84,8 @@ def _trains_plain_table(mod: Any) -> bool:
 
 def _walk(inner: Any, input_ids: torch.Tensor, mask: Any) -> torch.Tensor:
     table = inner.embed_tokens
-    if _trains_plain_table(table) and input_ids.device == table.weight.device:
-        h = embedding_lookup(input_ids, table.weight, padding_idx=table.padding_idx)
+    if _trains_plain_table(table):
+        h = module_lookup(table, input_ids)
     else:
         h = table(input_ids)
     b, length = input_ids.shape

@@ -1,7 +1,7 @@
 """`embedding_lookup`: scaled rows of a table, and the table's gradient by sorted tokens (csrc/embedding.cu).
 
-The reference's trunk calls the model's own embedding module (adapters/mlx_lm.py:140-164); the adapters here use this
-operator where the table is trained.  The gradient adds the rows of equal ids in fp32 and in a fixed order, rounds
+The reference's trunk calls the model's own embedding module (adapters/mlx_lm.py:140-164), and so do the adapters here; where
+the table is trained its gradient is this operator's.  The gradient adds the rows of equal ids in fp32 and in a fixed order, rounds
 once, and is the same bits for equal calls.
 """
 from __future__ import annotations
@@ -39,14 +39,14 @@ def _look_up(weight: torch.Tensor, ids: torch.Tensor, scale: float, padding: int
 
 
 class _Lookup(torch.autograd.Function):
-    """(weight, (ids, scale, padding)) -> ids.shape + (D,)."""
+    """(weight, (ids, scale, padding, rows or None)) -> ids.shape + (D,)."""
 
     @staticmethod
     def forward(ctx, weight, call):
-        ids, scale, padding = call
+        ids, scale, padding, rows = call
         ctx.save_for_backward(ids)
         ctx.rule = *weight.shape, weight.dtype, scale, padding
-        return _look_up(weight, ids, scale, padding)
+        return _look_up(weight, ids, scale, padding) if rows is None else rows
 
     @staticmethod
     def backward(ctx, d_out):
@@ -104,5 +104,14 @@ def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 
     if not ids.is_contiguous():
         ids = ids.contiguous()
     if weight.requires_grad and torch.is_grad_enabled():
-        return _Lookup.apply(weight, (ids, float(scale), padding))
+        return _Lookup.apply(weight, (ids, float(scale), padding, None))
     return _look_up(weight, ids, float(scale), padding)     # without autograd's function around it: 6 us of some 17
+
+
+def module_lookup(mod: torch.nn.Embedding, ids: torch.Tensor) -> torch.Tensor:
+    """`mod(ids)` with `embedding_lookup`'s gradient for its table, for the adapters' walk.  The rows are the module's own forward's,
+    which also stops at an id outside the table as it always did; `ids` int32 or int64 beside the table."""
+    with torch.no_grad():
+        rows = mod(ids)
+    padding = -1 if mod.padding_idx is None else mod.padding_idx
+    return _Lookup.apply(mod.weight, (ids.contiguous(), 1.0, padding, rows))

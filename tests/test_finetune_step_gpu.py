@@ -151,6 +151,19 @@ def test_which_tables_the_walk_looks_up(cuda_device):
     assert isinstance(mod.weight, Sharded) and not torch_lm._trains_plain_table(mod)
 
 
+def test_the_walk_s_rows_are_the_module_s_own(monkeypatch):
+    """Its check of the ids among them: with a table that the walk trains, an id outside the vocabulary still stops the program."""
+    inner = torch.nn.Module()
+    inner.embed_tokens, inner.layers, inner.norm = torch.nn.Embedding(10, 4, padding_idx=2), torch.nn.ModuleList(), torch.nn.Identity()
+    monkeypatch.setattr(torch_lm, "_trains_plain_table", lambda mod: True)
+    ids = torch.tensor([[1, 2, 9], [0, 0, 3]])
+    rows = torch_lm._walk(inner, ids, None)
+    assert torch.equal(rows, inner.embed_tokens(ids)) and rows.requires_grad
+    for bad in (10, -1):
+        with pytest.raises(IndexError):
+            torch_lm._walk(inner, torch.tensor([[1, bad]]), None)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("where", ["instance", "class"])
 def test_a_forward_put_in_place_of_the_table_s_own(cuda_device, monkeypatch, where):
