@@ -47,7 +47,8 @@ extern "C" {
 #define B200TP_DEV_TIMEOUT_MMA 102
 #define B200TP_DEV_TIMEOUT_EPILOGUE 103
 #define B200TP_DEV_TIMEOUT_OTHER 104
-#define B200TP_DEV_BAD_INDEX 105       /* no wait: an embedding id outside the table */
+#define B200TP_DEV_BAD_INDEX 105       /* no wait: an embedding id outside the table.  A word keeps its first report, so give the
+                                        * embedding's calls a word of their own where a timed-out wait must not go unseen */
 
 /* implementation selectors */
 #define B200TP_IMPL_AUTO 0   /* tcgen05 path for bf16 (head_dim 128 for attention), SIMT otherwise */

@@ -11,7 +11,7 @@ import ctypes as C
 import torch
 
 from mlx_train_perf_b200 import _lib
-from mlx_train_perf_b200.core.loss import VJP_CALLS, device_status
+from mlx_train_perf_b200.core.loss import VJP_CALLS, index_status
 from mlx_train_perf_b200.errors import EmbeddingInputError
 
 _DTYPES = (torch.float32, torch.bfloat16)
@@ -33,7 +33,7 @@ def _look_up(weight: torch.Tensor, ids: torch.Tensor, scale: float, padding: int
                            padding)
     with _lib.on(dev):
         rc = _lib.load().b200tp_embedding_fwd(C.byref(a), rows.data_ptr(), out.data_ptr(), _lib.stream(dev),
-                                              device_status(dev).data_ptr())
+                                              index_status(dev).data_ptr())
     _lib.check(rc)
     return out
 
@@ -67,7 +67,7 @@ class _Lookup(torch.autograd.Function):
             nbytes = lib.b200tp_embedding_bwd_workspace_bytes(C.byref(a))     # goes by the device's SMs
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
             rc = lib.b200tp_embedding_bwd(C.byref(a), rows.data_ptr(), grad.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
-                                          _lib.stream(dev), device_status(dev).data_ptr())
+                                          _lib.stream(dev), index_status(dev).data_ptr())
         _lib.check(rc)
         return grad, None
 

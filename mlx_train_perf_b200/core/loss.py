@@ -185,20 +185,27 @@ def _validate_inputs(hidden: torch.Tensor, head: HeadRef, targets: torch.Tensor,
 # native calls
 # ---------------------------------------------------------------------------------------
 _status: dict[int, torch.Tensor] = {}
+_index_status: dict[int, torch.Tensor] = {}
 
 
 def device_status(device: torch.device) -> torch.Tensor:
     """Per-device int32 word the kernels write when a bounded wait gives up."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     if idx not in _status:
-        _status[idx] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        _status[idx], _index_status[idx] = torch.zeros(2, dtype=torch.int32, device=torch.device("cuda", idx)).split(1)
     return _status[idx]
 
 
+def index_status(device: torch.device) -> torch.Tensor:
+    """Per-device int32 word for embedding ids outside their table: not the waits', since only the first report of a word stays."""
+    device_status(device)
+    return _index_status[device.index if device.index is not None else torch.cuda.current_device()]
+
+
 def check_device_status(device: torch.device | None = None) -> None:
-    """Synchronise and raise `DeviceTimeoutError` if any kernel reported a timed-out wait (`EmbeddingInputError` for an embedding id
-    outside its table)."""
-    for idx, t in list(_status.items()):
+    """Synchronise and raise `DeviceTimeoutError` if any kernel reported a timed-out wait, else `EmbeddingInputError` if an embedding
+    id lay outside its table (behind a timed-out wait the next call raises that)."""
+    for idx, t in [*_status.items(), *_index_status.items()]:
         if device is not None and device.index is not None and idx != device.index:
             continue
         code = int(t.item())

@@ -9,8 +9,8 @@ import math
 import pytest
 import torch
 
-from mlx_train_perf_b200 import EmbeddingInputError, embedding_lookup
-from mlx_train_perf_b200.core.loss import check_device_status
+from mlx_train_perf_b200 import DeviceTimeoutError, EmbeddingInputError, _lib, embedding_lookup
+from mlx_train_perf_b200.core.loss import check_device_status, device_status
 
 pytestmark = pytest.mark.gpu
 
@@ -175,6 +175,22 @@ def test_padding_and_ids_outside_the_table(cuda_device):
     with pytest.raises(EmbeddingInputError, match="0 <= id < V"):
         embedding_lookup(wild, w, validate_ids=True)
     embedding_lookup(ids, w, validate_ids=True)
+
+
+def test_a_bad_id_does_not_hide_a_wait_that_ran_out(cuda_device):
+    """Both in one step, the bad id first (the wait is the library's self-test, which runs into its limit): both are reported, the wait
+    before the id, each once."""
+    dev = cuda_device
+    check_device_status()
+    embedding_lookup(torch.tensor([3, 99], device=dev), torch.zeros(10, 8, device=dev))
+    waited = torch.zeros(2, dtype=torch.int64, device=dev)
+    _lib.check(_lib.load().b200tp_selftest_bounded_wait(waited.data_ptr(), torch.cuda.current_stream(dev).cuda_stream,
+                                                        device_status(dev).data_ptr()))
+    with pytest.raises(DeviceTimeoutError):
+        check_device_status()
+    with pytest.raises(EmbeddingInputError, match="outside"):
+        check_device_status(dev)
+    check_device_status()
 
 
 def test_values_that_are_not_finite_stay_in_their_rows(cuda_device):
