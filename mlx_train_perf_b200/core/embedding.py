@@ -11,7 +11,7 @@ import ctypes as C
 import torch
 
 from mlx_train_perf_b200 import _lib
-from mlx_train_perf_b200.core.loss import VJP_CALLS, index_status
+from mlx_train_perf_b200.core.loss import VJP_CALLS, has_tangent, index_status
 from mlx_train_perf_b200.errors import EmbeddingInputError
 
 _DTYPES = (torch.float32, torch.bfloat16)
@@ -82,6 +82,8 @@ def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 
     shape = weight.shape
     if len(shape) != 2 or 0 in shape:
         raise EmbeddingInputError(f"weight must be (V, D), got {tuple(shape)}")
+    if has_tangent(weight):
+        raise EmbeddingInputError("embedding_lookup has no forward-mode derivative")
     if not weight.is_cuda:
         raise EmbeddingInputError(f"weight must be a CUDA tensor (the operator has no CPU path); got {weight.device}")
     if weight.dtype not in _DTYPES:

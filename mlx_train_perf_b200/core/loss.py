@@ -20,6 +20,7 @@ from dataclasses import dataclass
 from typing import Literal, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from mlx_train_perf_b200 import _lib
 from mlx_train_perf_b200.errors import LossInputError, UnsupportedHeadError
@@ -212,6 +213,12 @@ def check_device_status(device: torch.device | None = None) -> None:
         if code != 0:
             t.zero_()
             _lib.raise_for_device_status(code)
+
+
+def has_tangent(t: torch.Tensor) -> bool:
+    """Whether forward-mode differentiation goes through `t`.  Calls that leave autograd's function out where no gradient is recorded must
+    refuse it: on raw addresses the tangent would be lost without a word."""
+    return forward_ad.unpack_dual(t).tangent is not None
 
 
 def _dtype_code(dt: torch.dtype) -> int:

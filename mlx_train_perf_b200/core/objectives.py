@@ -19,7 +19,7 @@ from typing import Literal, NamedTuple
 import torch
 
 from mlx_train_perf_b200 import _lib
-from mlx_train_perf_b200.core.loss import VJP_CALLS
+from mlx_train_perf_b200.core.loss import VJP_CALLS, has_tangent
 from mlx_train_perf_b200.errors import LossInputError
 
 _PREFERENCES = {"sigmoid": 0, "hinge": 1, "squared": 2}
@@ -48,6 +48,8 @@ def _unit_inner(t: torch.Tensor) -> torch.Tensor:
 
 def _check_tokens(logps: torch.Tensor, cu_seqlens: torch.Tensor | None, validate_seqlens: bool) -> int:
     """The number of sequences."""
+    if has_tangent(logps):
+        raise LossInputError("this loss has no forward-mode derivative")
     if not logps.is_cuda:
         raise LossInputError(f"logps must be a CUDA tensor (the operators have no CPU path); got {logps.device}")
     if logps.dtype not in _DTYPES:

@@ -535,3 +535,21 @@ def test_with_the_vocabulary_loss(cuda_device):
         want.backward()
         assert abs(loss.item() - want.item()) < 5e-5 * max(1.0, abs(want.item()))
         assert (leaf.grad.double().cpu() - leaf64.grad).abs().max() <= 1e-2 * leaf64.grad.abs().max()
+
+
+def test_forward_mode_derivatives_are_refused(cuda_device):
+    """With and without a recorded gradient; beside a dual level a call without tangents gives what it gives outside."""
+    from torch.autograd import forward_ad
+    from mlx_train_perf_b200 import EmbeddingInputError, embedding_lookup
+    x = torch.randn(4, 30, generator=torch.Generator().manual_seed(1)).to(cuda_device)
+    a, ids = torch.ones(4, 1, device=cuda_device), torch.arange(4, device=cuda_device)
+    want = preference_loss(x).loss, policy_loss(x, x + 0.1, a).loss, embedding_lookup(ids, x)
+    for leaf in (x, x.clone().requires_grad_(True)):
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(leaf, torch.ones_like(x))
+            for call, error in ((lambda: preference_loss(dual), LossInputError), (lambda: policy_loss(dual, x, a), LossInputError),
+                                (lambda: embedding_lookup(ids, dual), EmbeddingInputError)):
+                with pytest.raises(error, match="forward-mode"):
+                    call()
+            got = preference_loss(x).loss, policy_loss(x, x + 0.1, a).loss, embedding_lookup(ids, x)
+            assert all(torch.equal(p, q) for p, q in zip(got, want))

@@ -175,6 +175,23 @@ def test_status_text(lib):
         _lib.raise_for_device_status(_lib.DEV_BAD_INDEX)
 
 
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor does not require a gradient, and its tangent must not vanish on the way."""
+    from torch.autograd import forward_ad
+    x, a = torch.zeros(2, 4), torch.zeros(2, 1)
+    for leaf in (x, torch.zeros(2, 4, requires_grad=True)):
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(leaf, torch.ones(2, 4))
+            with pytest.raises(LossInputError, match="forward-mode"):
+                preference_loss(dual)
+            with pytest.raises(LossInputError, match="forward-mode"):
+                policy_loss(dual, x, a)
+            with pytest.raises(EmbeddingInputError, match="forward-mode"):
+                embedding_lookup(torch.zeros(3, dtype=torch.int64), dual)
+            with pytest.raises(LossInputError, match="CUDA"):       # a tensor without a tangent is looked at as ever
+                preference_loss(x)
+
+
 def test_host_tensors_are_refused():
     x, a = torch.zeros(2, 4), torch.zeros(2, 1)
     with pytest.raises(LossInputError, match="CUDA"):
