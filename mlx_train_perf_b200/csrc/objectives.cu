@@ -342,7 +342,8 @@ policy_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ old, const
     if (!on) return 0.f;
     const float u = t.sign * (xv - ov);
     const bool up = a > 0.f && u > r.log_high, down = a < 0.f && u < r.log_low, clipped = up || down;
-    const float gain = a * (clipped ? (up ? r.high : r.low) : expf(u));
+    // without an advantage nothing, also where the ratio leaves fp32
+    const float gain = a == 0.f && u < INFINITY ? 0.f : a * (clipped ? (up ? r.high : r.low) : expf(u));
     float slope = clipped ? 0.f : -gain;
     float kl = 0.f;
     if constexpr (REF) {

@@ -553,3 +553,19 @@ def test_forward_mode_derivatives_are_refused(cuda_device):
                     call()
             got = preference_loss(x).loss, policy_loss(x, x + 0.1, a).loss, embedding_lookup(ids, x)
             assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("length", [5, 4000])
+def test_no_advantage_and_a_ratio_beyond_fp32(cuda_device, length):
+    """exp(100) is infinite in fp32; times an advantage of zero it is still nothing, and other tokens' losses stay.  A NaN that counts is
+    still one."""
+    dev = cuda_device
+    x = torch.zeros(2, length, device=dev, requires_grad=True)
+    old = torch.tensor([[-100.0], [0.0]], device=dev).expand(2, length).contiguous()
+    for a in (torch.tensor([[0.0], [1.0]], device=dev), torch.tensor([[-0.0], [1.0]], device=dev).expand(2, length).contiguous()):
+        got = policy_loss(x, old, a)
+        grad, = torch.autograd.grad(got.loss, x)
+        assert got.loss.item() == -0.5 and got.clip_fraction.item() == 0.0
+        assert (grad[0] == 0).all() and torch.allclose(grad[1], torch.full_like(grad[1], -0.5 / length), rtol=4 * E32, atol=0.0)
+    old[0, 1] = math.nan
+    assert torch.isnan(policy_loss(x, old, a).loss)
