@@ -418,7 +418,7 @@ typedef struct b200tp_adamw_args {
   int64_t step;                  /* of this step, from 1 */
   int32_t param_dtype, grad_dtype;
   int32_t bits;
-  int32_t reserved;              /* 0 */
+  int32_t check_only;            /* 0; 1: looks at the arguments and the tensors, and launches nothing */
 } b200tp_adamw_args;
 
 /* m = b1 m + (1 - b1) g; v = b2 v + (1 - b2) g g; p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps), in

@@ -81,7 +81,7 @@ class AdamwArgs(C.Structure):
         ("exp_avg_out", C.c_void_p), ("exp_avg_sq_out", C.c_void_p), ("scales_out", C.c_void_p), ("master_out", C.c_void_p),
         ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
         ("grad_scale", C.c_double), ("grad_scale_ptr", C.c_void_p), ("step", C.c_int64),
-        ("param_dtype", C.c_int32), ("grad_dtype", C.c_int32), ("bits", C.c_int32), ("reserved", C.c_int32),
+        ("param_dtype", C.c_int32), ("grad_dtype", C.c_int32), ("bits", C.c_int32), ("check_only", C.c_int32),
     ]
 
 

@@ -201,7 +201,11 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
     with _lib.on(dev):
         stream = _lib.stream(dev)
         numbers = {int(step)} if steps is None else set(steps)
-        for number in sorted(numbers):                   # tensors that took different numbers of steps: a launch for each number
+        if len(numbers) > 1:                             # tensors that took different numbers of steps: a launch for each number ...
+            a.step, a.check_only = 1, 1                  # ... but only if all tensors together pass
+            _lib.check(lib.b200tp_adamw_step(C.byref(a), rows.ctypes.data, len(rows), stream))
+            a.check_only = 0
+        for number in sorted(numbers):
             part = rows if len(numbers) == 1 else np.ascontiguousarray(rows[[s == number for s in steps]])
             a.step = number
             _lib.check(lib.b200tp_adamw_step(C.byref(a), part.ctypes.data, len(part), stream))

@@ -563,7 +563,7 @@ extern "C" int b200tp_adamw_step(const b200tp_adamw_args* a, const b200tp_adamw_
   try {
     int rc = check(a, tensors, count);
     if (rc) return rc;
-    if (count == 0) return B200TP_OK;
+    if (count == 0 || a->check_only != 0) return B200TP_OK;
     rc = require_sm100();
     if (rc) return rc;
     Rule r;

@@ -454,6 +454,19 @@ def test_tensors_that_share_memory_are_refused(cuda_device):
     adamw_step(touching, [g[:500], g[500:]], AdamWState.zeros(touching), **RULE)
 
 
+def test_tensors_of_different_ages_that_share_memory_are_refused(cuda_device):
+    """A launch for each age must not get round the check, nor move some tensors before another one is refused."""
+    dev = cuda_device
+    p = torch.ones(1000, device=dev)
+    g = [torch.ones(1000, device=dev), torch.ones(1000, device=dev)]
+    for pair, grads in (([p, p], g), ([p[:600], p[400:]], [g[0][:600], g[1][:600]]), ([p, torch.ones(1000, device=dev)], [g[0], p])):
+        state = AdamWState.zeros(pair)
+        state.steps = [0, 4]
+        with pytest.raises(OptimizerInputError, match="share memory"):
+            adamw_step(pair, grads, state, **RULE)
+        assert (p == 1).all() and state.steps == [0, 4] and (state.exp_avg == 0).all()
+
+
 def test_refusals(cuda_device):
     dev = cuda_device
     p, g = [torch.zeros(8, 4, device=dev)], [torch.zeros(8, 4, device=dev)]

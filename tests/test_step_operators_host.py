@@ -135,6 +135,12 @@ def test_addresses_of_many_tensors(lib):
     assert ask([good[0].to(torch.bfloat16)], dtype=1) == -1
 
 
+def test_adamw_check_alone(lib):
+    """Passes what would be launched, refuses what would be refused; with no GPU either way."""
+    assert _adamw([ROW, [PTR + 400, PTR + 400, PTR + 400, 100, 256]], check_only=1) == _lib.OK
+    assert _adamw([ROW, [PTR + 396, PTR + 400, PTR + 396, 100, 256]], check_only=1) == _lib.ERR_OPTIM_INPUT
+
+
 def test_adamw_of_nothing(lib):
     assert _adamw([]) == _lib.OK
 
