@@ -114,6 +114,41 @@ def test_order_of_the_sum_is_the_tokens_own(cuda_device):
     assert torch.equal(grad[2].cpu(), acc) and (grad[[0, 1, 3]] == 0).all()
 
 
+def _sums_in_order(ids, dy, v, window):
+    """Each row's sum in fp32 in the order that is promised beyond 64 tokens: tokens sorted by id, equal ids as they came; token by token
+    within a window of sorted tokens; of a run that crosses windows the first window's sum, then the others', in four shares of
+    adjacent windows whose sums are added in turn."""
+    order = torch.argsort(ids, stable=True)
+    out = torch.zeros(v, dy.shape[1])
+    add = lambda rows: sum(rows[1:], rows[0]) if rows else torch.zeros(dy.shape[1])
+    for key in ids.unique().tolist():
+        at = (ids[order] == key).nonzero()[:, 0].tolist()          # adjacent places in the sorted order
+        parts = {}
+        for i in at:
+            parts.setdefault(i // window, []).append(dy[order[i]])
+        first, *others = [add(rows) for _, rows in sorted(parts.items())]
+        each = (len(others) + 3) // 4
+        shares = [others[k * each:(k + 1) * each] for k in range(4)]
+        out[key] = add([add([first, *shares[0]]), *(add(s) for s in shares[1:])]) if others else first
+    return out
+
+
+@pytest.mark.parametrize("n,v,kind", [(65, 4, "uniform"), (65, 40, "uniform"), (72, 2, "uniform"), (200, 7, "words"), (700, 3, "one"), (1000, 60, "words"),
+                                      (1000, 700, "words")])
+def test_order_of_the_sum_beyond_64_tokens(cuda_device, n, v, kind):
+    """Bit for bit, with values from 1 to 2^24 so that another order gives another sum: sort, windows of 8 tokens (as many as a thousand
+    tokens take), and runs that cross them."""
+    dev = cuda_device
+    g = torch.Generator().manual_seed(n + v)
+    ids = _ids(n, v, kind, g)
+    dy = torch.randn(n, 16, generator=g) * 2.0 ** torch.randint(0, 25, (n, 16), generator=g)
+    want = _sums_in_order(ids, dy, v, 8)
+    assert not torch.equal(want, _sums_in_order(ids.flip(0), dy.flip(0), v, 8))    # the order shows
+    w = torch.zeros(v, 16, device=dev, requires_grad=True)
+    grad, = torch.autograd.grad(embedding_lookup(ids.to(dev), w), w, dy.to(dev))
+    assert torch.equal(grad.cpu(), want)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_shapes_types_and_strides(cuda_device, dtype):
     dev = cuda_device
