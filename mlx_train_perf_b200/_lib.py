@@ -210,12 +210,12 @@ def tensor_rows():
         _tensor_rows = False
         capsule = getattr(torch.Tensor, "__dlpack_c_exchange_api__", None)
         if capsule is not None:
-            get = C.pythonapi.PyCapsule_GetPointer
-            get.restype, get.argtypes = C.c_void_p, [C.py_object, C.c_char_p]
+            # a prototype of its own: `ctypes.pythonapi`'s functions are shared by the whole process
+            get = C.PYFUNCTYPE(C.c_void_p, C.py_object, C.c_char_p)(("PyCapsule_GetPointer", C.pythonapi))
             table = get(capsule, b"dlpack_exchange_api")
-            if C.c_uint32.from_address(table).value == 1:
-                # two words of header, then the allocator, two functions for owning exchange, and the one wanted here
-                describe = C.c_void_p.from_address(table + 5 * C.sizeof(C.c_void_p)).value
+            # two words of header, then the allocator, two functions for owning exchange, and the one wanted here, which may be missing
+            describe = C.c_void_p.from_address(table + 5 * C.sizeof(C.c_void_p)).value
+            if C.c_uint32.from_address(table).value == 1 and describe:
                 fn = C.PyDLL(str(LIB_PATH)).b200tp_tensor_rows            # keeps the interpreter's lock
                 fn.restype, fn.argtypes = SIGNATURES["b200tp_tensor_rows"]
                 _tensor_rows = partial(fn, describe)

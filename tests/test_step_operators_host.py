@@ -135,6 +135,19 @@ def test_addresses_of_many_tensors(lib):
     assert ask([good[0].to(torch.bfloat16)], dtype=1) == -1
 
 
+def test_exchange_tables_without_what_is_wanted(lib, monkeypatch):
+    """A table that leaves the function out, or one of another version: tensors are then asked one by one.  The process's own
+    prototypes stay as they are."""
+    new = C.PYFUNCTYPE(C.py_object, C.c_void_p, C.c_char_p, C.c_void_p)(("PyCapsule_New", C.pythonapi))
+    monkeypatch.setattr(C.pythonapi.PyCapsule_GetPointer, "restype", C.c_int)
+    for version, entry in ((1, 0), (2, PTR), (1, PTR)):
+        table = (C.c_uint64 * 8)(version, 0, 1, 1, 1, entry, 0, 0)
+        monkeypatch.setattr(torch.Tensor, "__dlpack_c_exchange_api__", new(C.addressof(table), b"dlpack_exchange_api", None), raising=False)
+        monkeypatch.setattr(_lib, "_tensor_rows", None)
+        assert (_lib.tensor_rows() is None) == (version != 1 or not entry)
+    assert C.pythonapi.PyCapsule_GetPointer.restype is C.c_int
+
+
 def test_adamw_check_alone(lib):
     """Passes what would be launched, refuses what would be refused; with no GPU either way."""
     assert _adamw([ROW, [PTR + 400, PTR + 400, PTR + 400, 100, 256]], check_only=1) == _lib.OK
