@@ -427,7 +427,13 @@ adamw_kernel(const __grid_constant__ Table<N> table, const States st, const Rule
         v[e] = fmaf(r.beta2, v[e], r.one_beta2 * a * a);
         pv[e] = fmaf(pv[e], r.decay, -r.rate * __fdividef(m[e], fmaf(sqrtf(v[e]), r.root, r.eps)));
       }
-      if constexpr (MASTER) store8(st.master_out + j, true, 8, pv);
+      if constexpr (MASTER) {
+        if (n < 8) {                                                // padding stays zero, which 0 / (0 + eps) is not without an eps
+#pragma unroll
+          for (int e = 0; e < 8; ++e) pv[e] = e < n ? pv[e] : 0.f;
+        }
+        store8(st.master_out + j, true, 8, pv);
+      }
       store8(out + i, p_vec, n, pv);
       store8(static_cast<float*>(st.m_out) + j, true, 8, m);
       store8(static_cast<float*>(st.v_out) + j, true, 8, v);

@@ -117,6 +117,20 @@ def test_step(cuda_device, bits, p_dtype, g_dtype, master, scale):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+def test_what_lies_behind_a_tensor_stays_zero_without_eps(cuda_device, bits):
+    """0 / (0 + 0) of elements that are not there must not get into the masters' padding."""
+    params, grads = _tensors(SHAPES, torch.bfloat16, cuda_device, 1), _tensors(SHAPES, torch.bfloat16, cuda_device, 2)
+    state = AdamWState.zeros(params, bits=bits, master=True)
+    for _ in range(2):
+        adamw_step(params, grads, state, lr=0.1, eps=0.0)
+    for i, n in enumerate(state.numels):
+        o = int(state.rows[i, 4])
+        for flat in (state.master, state.exp_avg, state.exp_avg_sq):
+            assert (flat[o + n:o + (n + 255) // 256 * 256].float() == 0).all()
+    assert torch.isfinite(state.master).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("master", [False, True])
 def test_other_buffers_get_what_the_step_in_place_gives(cuda_device, bits, master):
     dev = cuda_device
