@@ -519,8 +519,9 @@ int check(const b200tp_adamw_args* a, const b200tp_adamw_tensor* t, int32_t coun
   if (!(a->beta1 >= 0. && a->beta1 < 1.) || !(a->beta2 >= 0. && a->beta2 < 1.)) return fail(B200TP_ERR_OPTIM_INPUT, "betas must lie in [0, 1)");
   if (!(a->eps >= 0.) || !(a->lr >= 0.) || !(a->weight_decay >= 0.))
     return fail(B200TP_ERR_OPTIM_INPUT, "lr, eps and weight_decay must not be negative");
-  if (count > 0 && (a->exp_avg == nullptr || a->exp_avg_sq == nullptr || a->exp_avg_out == nullptr || a->exp_avg_sq_out == nullptr ||
-                    (a->bits == 8 && (a->scales == nullptr || a->scales_out == nullptr))))
+  const bool some = std::any_of(t, t + count, [](const b200tp_adamw_tensor& x) { return x.numel != 0; });
+  if (some && (a->exp_avg == nullptr || a->exp_avg_sq == nullptr || a->exp_avg_out == nullptr || a->exp_avg_sq_out == nullptr ||
+               (a->bits == 8 && (a->scales == nullptr || a->scales_out == nullptr))))
     return fail(B200TP_ERR_OPTIM_INPUT, "null states");
   const void* states[] = {a->exp_avg, a->exp_avg_sq, a->scales, a->master, a->exp_avg_out, a->exp_avg_sq_out, a->scales_out, a->master_out};
   for (const void* p : states)

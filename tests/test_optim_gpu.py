@@ -456,6 +456,18 @@ def test_offsets_beyond_32_bits(cuda_device, bits):
         assert state.exp_avg.float()[at].item() * (0.5 - k % 2) > 0 if bits == 8 else state.exp_avg[at].item() == pytest.approx(0.1 * (0.5 - k % 2))
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_tensors_without_elements_alone(cuda_device, bits):
+    """A group of one dtype may hold nothing else; they count their steps like any other.  The other group moves by half, of which 16 x 2^-24
+    may be missing (as above) and 1e-8 to eps; 3 x 2^-24 of 1 for the parameter."""
+    p = torch.nn.Parameter(torch.zeros(0, 5, dtype=torch.bfloat16, device=cuda_device))
+    q = torch.nn.Parameter(torch.ones(3, device=cuda_device))
+    opt = AdamW([p, q], lr=0.5, weight_decay=0.0, bits=bits, master=True)
+    p.grad, q.grad = torch.zeros_like(p), torch.ones_like(q)
+    opt.step()
+    assert (q - 0.5).abs().max().item() <= 0.5 * (16 * E32 + 1e-8) + 3 * E32 and [s["step"] for s in opt.state_dict()["state"].values()] == [1, 1]
+
+
 def test_tensors_that_share_memory_are_refused(cuda_device):
     dev = cuda_device
     p = torch.zeros(1000, device=dev)
