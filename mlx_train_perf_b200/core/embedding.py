@@ -115,5 +115,5 @@ def module_lookup(mod: torch.nn.Embedding, ids: torch.Tensor) -> torch.Tensor:
     which also stops at an id outside the table as it always did; `ids` int32 or int64 beside the table."""
     with torch.no_grad():
         rows = mod(ids)
-    padding = -1 if mod.padding_idx is None else mod.padding_idx
+    padding = -1 if mod.padding_idx is None else mod.padding_idx % mod.weight.shape[0]
     return _Lookup.apply(mod.weight, (ids.contiguous(), 1.0, padding, rows))

@@ -165,6 +165,24 @@ def test_the_walk_s_rows_are_the_module_s_own(monkeypatch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("padding", [None, 3, 9, -1, -10])
+def test_the_walk_s_table_gradient(cuda_device, padding):
+    """The module's own rows with the package's gradient, a padding id given from either end; whole numbers, so that sums are exact."""
+    inner = torch.nn.Module()
+    inner.embed_tokens, inner.layers, inner.norm = torch.nn.Embedding(10, 8).to(cuda_device), torch.nn.ModuleList(), torch.nn.Identity()
+    table = inner.embed_tokens
+    table.padding_idx = padding
+    for rows in (2, 40):
+        ids = torch.randint(0, 10, (rows, 5), generator=torch.Generator().manual_seed(rows)).to(cuda_device)
+        dy = torch.randint(-4, 5, (rows, 5, 8), generator=torch.Generator().manual_seed(3)).float().to(cuda_device)
+        calls = VJP_CALLS.get("embedding_lookup", 0)
+        out = torch_lm._walk(inner, ids, None)
+        got, = torch.autograd.grad(out, table.weight, dy)
+        want, = torch.autograd.grad(torch.nn.functional.embedding(ids, table.weight, padding_idx=padding), table.weight, dy)
+        assert torch.equal(out, table(ids)) and torch.equal(got, want) and VJP_CALLS["embedding_lookup"] == calls + 1
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("where", ["instance", "class"])
 def test_a_forward_put_in_place_of_the_table_s_own(cuda_device, monkeypatch, where):
     """As tools that wrap modules in place do it: the walk's rows are that function's, and so is the table's gradient."""
