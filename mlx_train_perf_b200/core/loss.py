@@ -193,7 +193,8 @@ def device_status(device: torch.device) -> torch.Tensor:
     """Per-device int32 word the kernels write when a bounded wait gives up."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     if idx not in _status:
-        _status[idx], _index_status[idx] = torch.zeros(2, dtype=torch.int32, device=torch.device("cuda", idx)).split(1)
+        with torch.inference_mode(False):                # the first call may come in inference mode; clearing a word need not
+            _status[idx], _index_status[idx] = torch.zeros(2, dtype=torch.int32, device=torch.device("cuda", idx)).split(1)
     return _status[idx]
 
 

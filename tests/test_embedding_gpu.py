@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from mlx_train_perf_b200 import DeviceTimeoutError, EmbeddingInputError, _lib, embedding_lookup
+from mlx_train_perf_b200.core import loss
 from mlx_train_perf_b200.core.loss import check_device_status, device_status
 
 pytestmark = pytest.mark.gpu
@@ -225,6 +226,17 @@ def test_a_bad_id_does_not_hide_a_wait_that_ran_out(cuda_device):
         check_device_status()
     with pytest.raises(EmbeddingInputError, match="outside"):
         check_device_status(dev)
+    check_device_status()
+
+
+def test_a_bad_id_of_the_first_call_in_inference_mode(cuda_device, monkeypatch):
+    """The words that are made in that call can be read and cleared outside it."""
+    for words in ("_status", "_index_status"):
+        monkeypatch.setattr(loss, words, {})
+    with torch.inference_mode():
+        embedding_lookup(torch.tensor([3, 99], device=cuda_device), torch.zeros(10, 8, device=cuda_device))
+    with pytest.raises(EmbeddingInputError, match="outside"):
+        check_device_status()
     check_device_status()
 
 
