@@ -403,7 +403,10 @@ typedef struct b200tp_adamw_args {
   /* States, flat over all tensors, each tensor's share padded to a multiple of 256 elements (padding zero); 16-byte
    * aligned; *_out may be the same buffers (a step in place) or others that do not overlap them.
    * bits 32: exp_avg, exp_avg_sq f32.  bits 8: e4m3 codes of m and of sqrt(v), and scales (blocks of 256, 2) f32:
-   * m = code * scales[.][0], sqrt(v) = code * scales[.][1]. */
+   * m = code * scales[.][0], sqrt(v) = code * scales[.][1].  sqrt(v), and m where rounding to nearest could hold a code
+   * that no gradient feeds (codes below 2^-6; with beta1 above 0.9 all), go up or down by a dither of position and step.
+   * m up to 1e-30 and sqrt(v) up to 4e-19 are held as zero.  An element one of whose moments is not finite (v overflows
+   * where 32 bits leave the parameter alone) gets NaN for both and for its parameter. */
   const void* exp_avg;
   const void* exp_avg_sq;
   const void* scales;

@@ -20,8 +20,10 @@
 // mantissa 8 to 15 falls by 0.8 to 1.5 of a distance (half as wide below 8) and is never rounded back; up to beta1 = 0.9 these go to
 // nearest.  Below 2^-6 the distance stays 2^-9, and code 4 comes back from 3.6: codes there are dithered wherever the gradient
 // adds less than 2^-6 too.  Above beta1 = 0.9 every m is dithered (at 0.95 code 9 comes back from 8.55).  A warp that meets an old
-// code below 2^-6 takes a form of the step that looks; all others ask once for eight elements.  789 M elements, sustained: 1427 us
-// (1395 with every m to nearest), 1850 us with all dithered.
+// code below 2^-6 takes a form of the step that looks; all others ask once for eight elements.  789 M elements, sustained: 1405 to
+// 1430 us (1345 to 1395 with every m to nearest), 1790 to 1850 us with all dithered.
+//
+// Moments of 1e-30 and less, and roots of 4e-19 and less, are held as zero: the factor to their codes would overflow.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
@@ -183,7 +185,8 @@ __device__ __forceinline__ Pair decode2(uint32_t w, int upper) {
   return Pair{f.x, f.y};
 }
 
-// 32 mixed bits of a pair of positions and the step: xor-shifts and odd multipliers.
+// 32 mixed bits of a pair of positions and the step: xor-shifts by 16, 15, 16 and multipliers between them, which are those of
+// C. Wellons's published search for 32-bit integer hashes of low bias (2018), the last one's top bit cleared.
 __device__ __forceinline__ uint32_t mix(uint32_t pair, uint32_t step) {
   uint32_t x = (pair + step * 0x3504F333u) * 0x1E3779B1u;
   x = (x ^ (x >> 16)) * 0x7FEB352Du;
