@@ -11,7 +11,8 @@ holds.  8-bit moments take 2 bytes a parameter and 8 for every 256: e4m3 codes o
 block of 256 elements; sqrt(v), and m wherever rounding to nearest could hold a value that no gradient feeds (small codes; with
 beta1 above 0.9 all of them), is rounded up or down by a dither fixed by position and step, so every rank of a data-parallel run gets
 the same codes.  They hold m up to 1e-30 and sqrt(v) up to 4e-19 as zero, and an element with a moment that is not finite gets NaN for
-both and for its parameter.  beta1 above 0.9 takes a third more time.
+both and for its parameter.  Moments, scales and codes are bit for bit those of fp32 operations rounded one by one, in the order written
+here.  beta1 above 0.9 takes a third more time.
 """
 from __future__ import annotations
 

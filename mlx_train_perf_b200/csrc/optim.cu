@@ -4,8 +4,8 @@
 // Everything is read once and written once: 28 bytes an element for bf16 parameters with fp32 masters and fp32 moments, 10 for
 // bf16 parameters with 8-bit moments.  HBM bounds the first.  The second leaves time for about 56 instructions an element at
 // HBM's rate, and written plainly (a rounded square root and quotient, selections for values that are not finite) it takes 79; so its
-// arithmetic works on pairs of fp32 values (fma.rn.f32x2), folds the scales into the factors, and tests a thread's eight
-// elements together for what is rare.
+// arithmetic works on pairs of fp32 values (fma.rn.f32x2), takes roots and quotients from approximate ones with one corrected step,
+// and tests a thread's eight elements together for what is rare.
 //
 // The table of tensors travels in the launch's own parameters: no copy to the device, no workspace, nothing that two captured
 // graphs would share.  A CTA takes some thousands of elements of one tensor; a warp takes blocks of 256, the elements that share a scale.
@@ -20,8 +20,12 @@
 // mantissa 8 to 15 falls by 0.8 to 1.5 of a distance (half as wide below 8) and is never rounded back; up to beta1 = 0.9 these go to
 // nearest.  Below 2^-6 the distance stays 2^-9, and code 4 comes back from 3.6: codes there are dithered wherever the gradient
 // adds less than 2^-6 too.  Above beta1 = 0.9 every m is dithered (at 0.95 code 9 comes back from 8.55).  A warp that meets an old
-// code below 2^-6 takes a form of the step that looks; all others ask once for eight elements.  789 M elements, sustained: 1405 to
-// 1430 us (1345 to 1395 with every m to nearest), 1790 to 1850 us with all dithered.
+// code below 2^-6 takes a form of the step that looks; all others ask once for eight elements.  789 M elements: 1263 us at full
+// clocks; sustained at the power cap 1475 us (1435 with every m to nearest), 1935 us with all dithered.
+//
+// Moments, roots, scales and codes are, bit for bit, those of the definition computed in fp32 with each operation rounded by itself:
+// codes depend on the last bit of what is rounded, so anything else gives other codes here and there (sums fused with
+// their products: 64 codes of m in 56 M; scales folded into the factors besides would be 4 % faster).
 //
 // Moments of 1e-30 and less, and roots of 4e-19 and less, are held as zero: the factor to their codes would overflow.
 #include <cuda_bf16.h>
@@ -54,7 +58,6 @@ constexpr int kFew = 48;                    // of the small form: 2 kB, 5.9 us o
 
 struct Rule {
   float beta1, beta2, one_beta1, one_beta2;
-  float root_beta2, root_one_beta2;         // of beta2 and 1 - beta2
   float eps, decay;                         // decay: 1 - lr weight_decay
   float rate;                               // lr / (1 - beta1^t)
   float root;                               // 1 / sqrt(1 - beta2^t)
@@ -159,6 +162,8 @@ __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits_of(a)), "l"(bits_of(b)));
   return pair_of(d);
 }
+// Two scalar additions: a packed one is fused with the product before it, which then goes unrounded.
+__device__ __forceinline__ Pair add2(Pair a, Pair b) { return Pair{__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)}; }
 __device__ __forceinline__ float rsqrt_ftz(float v) {
   float q;
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(v));
@@ -170,11 +175,10 @@ __device__ __forceinline__ float rcp_ftz(float v) {
   return q;
 }
 
-// 448 / v to half an ulp: the product with an approximate reciprocal, corrected by its exact remainder.  All codes of a block depend on
-// it.  (The reciprocal with a Newton step and then times 448 is two roundings.)
-__device__ __forceinline__ float over(float v) {
-  const float q = rcp_ftz(v), x = 448.f * q;
-  return fmaf(fmaf(-v, x, 448.f), q, x);
+// a / b rounded once, from an approximate reciprocal of b: the product corrected by its exact remainder.
+__device__ __forceinline__ Pair divide2(Pair a, Pair minus_b, Pair over_b) {
+  const Pair q = mul2(a, over_b);
+  return fma2(fma2(q, minus_b, a), over_b, q);
 }
 constexpr float kNoRoot = 4e-19f;           // roots up to here stand for zero: the root of 1e-37 is 3.2e-19
 
@@ -232,29 +236,28 @@ __device__ __forceinline__ void unpack(const Raw8<float>& r, Pair (&v)[4]) {
 }
 
 // 8-bit moments of eight elements: (codes, scales) and gradients in, parameters moved, (codes, scales) out.
-// m = beta1 sm code + one_beta1 g;  v = (sqrt(beta2) sv code)^2 + (sqrt(one_beta2) g)^2, g times grad_scale;  sqrt(v) from v rsqrt(v) and
-// one Newton step (about an ulp).  1e-37 is added to v, which keeps rsqrt finite and changes no v above 1e-30; what is then below
-// 1.6e-37 is zero.  `pair`: half the first element's place in the states, which fixes the dither.  LOOK: m that is not to go to
-// nearest is dithered, with the bits of the complement of `pair`.
+// m = beta1 (sm code) + one_beta1 g;  v = beta2 (sr code)^2 + (one_beta2 g) g, g times grad_scale before;  sqrt(v) from v rsqrt(v) and
+// one Newton step with the exact remainder.  1e-37 is added to the old v, which keeps rsqrt finite and changes no v above 1e-30; what is
+// then below 1.6e-37 is zero.  `pair`: half the first element's place in the states, which fixes the dither.  LOOK: m that is not to
+// go to nearest is dithered, with the bits of the complement of `pair`.
 template <bool LOOK>
-__device__ __forceinline__ void step8(uint2& mc, uint2& vc, float2& sc, const Pair (&g)[4], Pair (&p)[4], float grad_scale,
-                                      const Rule& r, uint32_t pair) {
+__device__ __forceinline__ void step8(uint2& mc, uint2& vc, float2& sc, const Pair (&g)[4], Pair (&p)[4], const Rule& r,
+                                      uint32_t pair) {
   Pair m[4], root[4];
-  const Pair bm = both(r.beta1 * sc.x), bv = both(r.root_beta2 * sc.y);
-  const Pair gm = both(r.one_beta1 * grad_scale), gr = both(r.root_one_beta2 * grad_scale);
+  const Pair old_m = both(sc.x), old_r = both(sc.y);
   float ma = 0.f;
   uint32_t top = 0, by_dither = 0;                                  // by_dither: bit k for element k
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const Pair cm = decode2(i < 2 ? mc.x : mc.y, i & 1), cv = decode2(i < 2 ? vc.x : vc.y, i & 1);
-    m[i] = fma2(g[i], gm, mul2(cm, bm));
+    const Pair fed = mul2(g[i], both(r.one_beta1));
+    m[i] = add2(mul2(mul2(cm, old_m), both(r.beta1)), fed);
     if constexpr (LOOK) {
-      const Pair fed = mul2(g[i], gm);
       if (r.dither_m || (fabsf(cm.x) < 0x1p-6f && fabsf(fed.x) < 0x1p-6f * sc.x)) by_dither |= 1u << (2 * i);
       if (r.dither_m || (fabsf(cm.y) < 0x1p-6f && fabsf(fed.y) < 0x1p-6f * sc.x)) by_dither |= 2u << (2 * i);
     }
-    const Pair new_root = mul2(g[i], gr), old_root = mul2(cv, bv);
-    const Pair v = fma2(new_root, new_root, fma2(old_root, old_root, both(1e-37f)));
+    const Pair old_root = mul2(cv, old_r);
+    const Pair v = add2(fma2(mul2(old_root, old_root), both(r.beta2), both(1e-37f)), mul2(mul2(g[i], both(r.one_beta2)), g[i]));
     const Pair q = Pair{rsqrt_ftz(v.x), rsqrt_ftz(v.y)};
     const Pair t = mul2(v, q);
     root[i] = fma2(Pair{fmaf(-t.x, t.x, v.x), fmaf(-t.y, t.y, v.y)}, mul2(q, both(0.5f)), t);
@@ -287,20 +290,20 @@ __device__ __forceinline__ void step8(uint2& mc, uint2& vc, float2& sc, const Pa
   float mm = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(ma))), rm = __uint_as_float(top);
   mm = mm > 1e-30f ? mm : 0.f;
   rm = rm > kNoRoot ? rm : 0.f;
-  const Pair mi = both(mm > 0.f ? over(mm) : 0.f), ri = both(rm > 0.f ? over(rm) : 0.f);
   sc = make_float2(mm * (1.f / 448.f), rm * (1.f / 448.f));
+  const Pair mi = both(mm > 0.f ? rcp_ftz(sc.x) : 0.f), ri = both(rm > 0.f ? rcp_ftz(sc.y) : 0.f), ms = both(-sc.x), rs = both(-sc.y);
   uint32_t mw[4], vw[4], low = 0xffffffffu;
   Pair y[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    Pair x = mul2(m[i], mi);
+    Pair x = divide2(m[i], ms, mi);
     if constexpr (LOOK) {
       const uint32_t bits = mix(~(pair + i), r.step);
       if (by_dither >> (2 * i) & 1) x.x = copysignf(dithered(fabsf(x.x), ((bits & 0xffffu) << 4) | 8u), x.x);
       if (by_dither >> (2 * i) & 2) x.y = copysignf(dithered(fabsf(x.y), ((bits >> 16) << 4) | 8u), x.y);
     }
     mw[i] = __nv_cvt_float2_to_fp8x2(make_float2(x.x, x.y), __NV_SATFINITE, __NV_E4M3);
-    y[i] = mul2(root[i], ri);
+    y[i] = divide2(root[i], rs, ri);
     low = min(low, min(__float_as_uint(y[i].x), __float_as_uint(y[i].y)));
   }
   mc = make_uint2(mw[0] | (mw[1] << 16), mw[2] | (mw[3] << 16));
@@ -391,13 +394,16 @@ adamw_kernel(const __grid_constant__ Table<N> table, const States st, const Rule
         constexpr int kStep = kThreads * 8;
         Pair gv[4], pv[4];
         unpack(gr[it], gv);
+        if (grad_scale != 1.f)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) gv[i] = mul2(gv[i], both(grad_scale));
         unpack(pr[it], pv);
         const uint32_t pair = static_cast<uint32_t>(j0 >> 1) + it * (kStep / 2);
         // top bit of a byte: the old code's exponent is not zero, so m is 2^-6 or more
         constexpr uint32_t kExp = 0x78787878u, kTop = 0x80808080u;
         const uint32_t normal = ((mc[it].x & kExp) + kExp) & ((mc[it].y & kExp) + kExp) & kTop;
-        if (__any_sync(0xffffffffu, normal != kTop || r.dither_m)) step8<true>(mc[it], vc[it], sc[it], gv, pv, grad_scale, r, pair);
-        else step8<false>(mc[it], vc[it], sc[it], gv, pv, grad_scale, r, pair);
+        if (__any_sync(0xffffffffu, normal != kTop || r.dither_m)) step8<true>(mc[it], vc[it], sc[it], gv, pv, r, pair);
+        else step8<false>(mc[it], vc[it], sc[it], gv, pv, r, pair);
         const float flat[8] = {pv[0].x, pv[0].y, pv[1].x, pv[1].y, pv[2].x, pv[2].y, pv[3].x, pv[3].y};
         if constexpr (MASTER) store8(st.master_out + j0 + it * kStep, true, 8, flat);
         store8(op + it * kStep, whole || p_vec, mine(it), flat);
@@ -581,8 +587,6 @@ extern "C" int b200tp_adamw_step(const b200tp_adamw_args* a, const b200tp_adamw_
     r.beta2 = static_cast<float>(a->beta2);
     r.one_beta1 = static_cast<float>(1. - a->beta1);
     r.one_beta2 = static_cast<float>(1. - a->beta2);
-    r.root_beta2 = static_cast<float>(std::sqrt(a->beta2));
-    r.root_one_beta2 = static_cast<float>(std::sqrt(1. - a->beta2));
     r.eps = static_cast<float>(a->eps);
     r.decay = static_cast<float>(1. - a->lr * a->weight_decay);
     r.rate = static_cast<float>(a->lr / (1. - std::pow(a->beta1, static_cast<double>(a->step))));
