@@ -569,3 +569,19 @@ def test_no_advantage_and_a_ratio_beyond_fp32(cuda_device, length):
         assert (grad[0] == 0).all() and torch.allclose(grad[1], torch.full_like(grad[1], -0.5 / length), rtol=4 * E32, atol=0.0)
     old[0, 1] = math.nan
     assert torch.isnan(policy_loss(x, old, a).loss)
+
+
+@pytest.mark.parametrize("length", [64, 5000])
+def test_a_kl_term_beside_gains_that_cancel(cuda_device, length):
+    """Tokens in pairs that differ in the sign of their advantage alone: what is left of the loss is the KL term, with its own roundings
+    (4 x 2^-24 as above, half of it for the result) and none of the gains', which are 10^5 times larger."""
+    dev = cuda_device
+    g = torch.Generator().manual_seed(5)
+    x = -torch.rand(2, length, generator=g).repeat_interleave(2, 1)
+    old = x + 0.02 * torch.rand(2, length, generator=g).repeat_interleave(2, 1)
+    ref = x + 0.03 * torch.randn(2, length, generator=g).repeat_interleave(2, 1)
+    a = torch.randn(2, length, generator=g).repeat_interleave(2, 1) * torch.tensor([1.0, -1.0]).repeat(length)
+    z = (ref - x).double()                                         # the kernel's own difference, rounded once
+    want = (torch.expm1(z) - z).mean().item() * 0.04
+    got = policy_loss(x.to(dev), old.to(dev), a.to(dev), ref_logps=ref.to(dev), kl_coef=0.04)
+    assert want < 1e-4 and abs(got.loss.item() - want) <= 6 * E32 * want and abs(got.kl.item() * 0.04 - want) <= 6 * E32 * want
