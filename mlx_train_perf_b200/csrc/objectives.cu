@@ -329,7 +329,7 @@ policy_tokens_kernel(const TX* __restrict__ x, const TR* __restrict__ old, const
   }
   int lo, hi;
   share(t, s, k, lo, hi);
-  // rows, so that the loop indexes with 32 bits (126 instructions a token with 64, 100 with 32, 81 four tokens at a time)
+  // rows, so that the loop indexes with 32 bits (126 instructions a token with 64, 100 with 32, 86 four tokens at a time)
   const TX* x_row = x + s * t.x_stride;
   const TR* old_row = old + s * t.old_stride;
   const TR* ref_row = REF ? ref + s * t.ref_stride : nullptr;
