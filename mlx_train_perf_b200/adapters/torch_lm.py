@@ -63,7 +63,11 @@ def split_model(model: Any) -> tuple[Callable[[torch.Tensor], torch.Tensor], Hea
     return trunk, head
 
 
-_EMBEDDING_FORWARD = torch.nn.Embedding.forward
+def _has_own_forward(mod: torch.nn.Embedding) -> bool:
+    """Whether calling `mod` runs torch's own code: no `forward` on the instance, and none put in the class's place at any time, this
+    module's import included."""
+    code = getattr(torch.nn.Embedding.forward, "__code__", None)
+    return "forward" not in vars(mod) and code is not None and code.co_filename == torch.nn.modules.sparse.__file__
 
 
 def _trains_plain_table(mod: Any) -> bool:
@@ -73,7 +77,7 @@ def _trains_plain_table(mod: Any) -> bool:
     module's own."""
     if type(mod) is not torch.nn.Embedding or not torch.is_grad_enabled() or _has_any_global_hook():
         return False
-    if "forward" in vars(mod) or torch.nn.Embedding.forward is not _EMBEDDING_FORWARD:
+    if not _has_own_forward(mod):
         return False
     w = mod.weight
     return (type(w) in (torch.Tensor, torch.nn.Parameter) and w.is_cuda and w.requires_grad and w.dtype in (torch.float32, torch.bfloat16)

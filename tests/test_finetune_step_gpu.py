@@ -3,6 +3,9 @@ loss, an objective, the backward pass and the optimizer's step; against the same
 elementary operations), fp32.  The attention and the vocabulary loss bound what may differ: 1e-3 of the largest gradient and 1e-4 of a
 loss, as in tests/test_wrapper_adapter.py."""
 import copy
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -162,6 +165,22 @@ def test_the_walk_s_rows_are_the_module_s_own(monkeypatch):
     for bad in (10, -1):
         with pytest.raises(IndexError):
             torch_lm._walk(inner, torch.tensor([[1, bad]]), None)
+
+
+def test_a_class_s_forward_replaced_before_the_import():
+    """Even by a function that carries the old one's name."""
+    code = """
+import functools, torch
+own = torch.nn.Embedding.forward
+if {replace}:
+    torch.nn.Embedding.forward = functools.wraps(own)(lambda self, ids: 3.0 * own(self, ids))
+from mlx_train_perf_b200.adapters import torch_lm
+print(torch_lm._has_own_forward(torch.nn.Embedding(3, 2)))
+"""
+    for replace in (True, False):
+        got = subprocess.run([sys.executable, "-c", code.format(replace=replace)], capture_output=True, text=True, check=True,
+                             cwd=Path(torch_lm.__file__).parents[2])
+        assert got.stdout.strip() == str(not replace)
 
 
 @pytest.mark.gpu
